@@ -14,50 +14,17 @@
 // online-softmax stream (m, l, acc) of its own; streams are merged by shuffles, waves
 // through LDS, partitions by attn_reduce.  Serves fp32 (every row) and bf16 (decode).
 // Plain reference: reference atomserve/kernels.py:167-334, atomserve/model.py:269-289.
-#include "common.h"
+#include "attn_parts.h"
 #include "no_alloc.h"
 #include <type_traits>
-
-#define NEG_INF (-__builtin_inff())
 
 // exp of the fp32 path is the precise one; bf16 serving uses the hardware approximation.
 template <typename T> __device__ __forceinline__ float fexp(float x);
 template <> __device__ __forceinline__ float fexp<float>(float x) { return expf(x); }
 template <> __device__ __forceinline__ float fexp<bf16>(float x) { return __expf(x); }
 
-// What a query at position p sees, and how scores become weights.
-struct Sight {
-  int window;  // > 0: keys p - window + 1 .. p; 0: every key up to p
-  int keep;    // with a window: the sequence's first `keep` keys stay visible behind it
-  int chunk;   // > 0: keys of the query's own chunk only, chunks of this many positions counted from 0 (without a window)
-  float cap;   // > 0: a score s counts as cap tanh(s / cap)
-  int sink;    // 1: the denominator has one more score, which has no value
-  const float* sinks;  // [H]: that score per query head (not scaled); null: 0 for all
-  int wide;    // 1: the kernels of bfloat16 heads write their results in fp32 (for a consumer that takes differences of them)
-};
-// The result of a head's coordinate i, in the type of the heads or in fp32 (`Sight::wide`).
-template <typename T>
-__device__ __forceinline__ void put(T* out, size_t i, float v, int wide) {
-  if (wide) reinterpret_cast<float*>(out)[i] = v;
-  else out[i] = from_f32<T>(v);
-}
-__device__ __forceinline__ int first_in_window(const Sight& sight, int ctx) {
-  if (sight.chunk > 0) return (ctx - 1) / sight.chunk * sight.chunk;
-  return sight.window > 0 ? max(0, ctx - sight.window) : 0;
-}
-__device__ __forceinline__ float sink_score(int sink, const float* sinks, int head) { return sink && sinks ? sinks[head] : 0.f; }
-static inline bool sight_ok(const Sight& s) {
-  return s.window >= 0 && s.keep >= 0 && (s.keep == 0 || s.window > 0) && s.cap >= 0.f && (s.sink == 0 || s.sink == 1) &&
-         (s.wide == 0 || s.wide == 1) && s.chunk >= 0 && (s.chunk == 0 || s.window == 0);
-}
 // Which instance of the matrix-core kernels computes it (`SEE` below).
 static inline int needed_sight(const Sight& s) { return s.cap > 0.f ? 2 : (s.keep > 0 || s.sink || s.wide || s.chunk > 0) ? 1 : 0; }
-
-// tanh through the hardware's exponential and reciprocal: an absolute error of 1e-7, which is what a capped score
-// (times the cap) of the bf16 kernels may carry.
-__device__ __forceinline__ float quick_tanh(float x) {
-  return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.8853900817779268f * x));
-}
 
 template <typename T> struct Chunk;  // 16 bytes of a head
 template <> struct Chunk<float> {
@@ -298,32 +265,10 @@ __global__ __launch_bounds__(256) void attn_reduce_kernel(const int* __restrict_
 //
 // The softmax weights are rounded to bf16 for the second product; maxima, sums and the
 // output accumulate in fp32.  Needs D % 32 == 0, D <= 256, block_size % 16 == 0.
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
-
 // Which of a step's 32 keys row `row` of its score tile `tile` (0, 1) stands for.  Rows 4g..4g+3
 // of both tiles are what lane group g holds after the score product, and they are keys
 // 8g .. 8g+7: eight neighbours, whose values are one 16-byte piece of a transposed page.
 #define KEY_OF_ROW(tile, row) (8 * ((row) >> 2) + ((row) & 3) + 4 * (tile))
-
-// Sums and maxima over the four lanes that share `lane % 16` (lane ^ 16, lane ^ 32) without a
-// trip through LDS: v_permlane16_swap / v_permlane32_swap exchange rows of 16 lanes between
-// two registers.  With both operands equal to x, the results hold (rows 0 0 2 2, rows 1 1 3 3)
-// and (rows 0 1 0 1, rows 2 3 2 3) of x.
-__device__ __forceinline__ float quad_rows_max(float v) {
-  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float quad_rows_sum(float v) {
-  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
 
 // The keys and values of one step (32 keys, two 16-key pieces of pages) of one kv head, as the
 // MFMA operands of this lane: keys as rows of A (16 bytes of the head of key KEY_OF_ROW(tile,
@@ -731,17 +676,7 @@ __global__ __launch_bounds__(256) void attn_decode_mfma_kernel(
 // A load instruction fills 64 consecutive slots (slot = first + lane); which 16 bytes of
 // memory a lane fetches is free, which is how the key layout comes about.
 // A query at position p sees keys lo..p by absolute position, wherever the row starts.
-// max(a, b, c) as the one instruction it is; NaN operands lose, as with fmaxf.
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-  return r;
-}
-
 #define PF_STAGES 4
-// s_waitcnt that only constrains the vector-memory counter (vmcnt: bits 3:0 and 15:14)
-#define PF_WAIT_VM(N) __builtin_amdgcn_s_waitcnt(((N) & 15) | (((N) >> 4) << 14) | (7 << 4) | (15 << 8))
-
 // A step of few work items takes as long as its longest one (a portion of a prompt behind thousands of cached
 // tokens: a hundred workgroups of hundreds of rounds each, on a GPU with room for five hundred).  With `pieces` > 1
 // every work item comes as that many workgroups: an item of more than `piece_rounds` rounds of 64 keys is cut
