@@ -1,0 +1,610 @@
+// A paged cache of keys and values in 8 bits, and attention over it.
+//
+// Pages of one layer hold e4m3 numbers, in blocks of 16 tokens that share a scale for each kv head:
+//
+//   k_pages  [num_pages, KV, bs, D]            a block of keys: 16 rows of D bytes
+//   v_pages  [num_pages, KV, bs / 16, D, 16]   a block of values, transposed: for every coordinate its 16 tokens
+//   scales   fp32 [num_pages, KV, bs / 16]     one for the keys and one for the values; a number is its e4m3 value times the scale
+//
+// A token at position p of a request lives in page table[p / bs] at offset p % bs, so that a block of either kind is 16 D bytes in one piece, at
+// the same place in both.  A block's scale is the power of two 2^e with the smallest e in -100 .. 119 for which its largest magnitude is at
+// most 448 * 2^e (448 is the largest e4m3 number).  A block is filled token by token while its scale grows, and what it holds is then
+// rewritten: times a power of two an e4m3 number stays the same number unless it falls under the smallest normal one (2^-15 of the
+// largest), so a block holds what a single rounding gives, however its tokens came.  Integers, or any scale, would be rounded anew each time.
+#include "attn_parts.h"
+
+namespace {
+
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+
+constexpr int BLOCK = 16;                // tokens that share a scale
+constexpr int LEAST = -100, MOST = 119;  // a scale's exponent: below, bf16 numbers would be no normal ones; above, 448 times it would be none
+constexpr float LARGEST = 448.f;
+constexpr float LOG2E = 1.4426950408889634f;
+
+// The scale of numbers of up to `amax` (finite): 448 is 1.75 * 2^8, and a mantissa beyond 1.75 carries into the exponent.
+__device__ __forceinline__ float block_scale(float amax) {
+  const int e = (int)((__float_as_uint(amax) + 0x1fffffu) >> 23) - 127 - 8;
+  return __uint_as_float((unsigned)(min(max(e, LEAST), MOST) + 127) << 23);
+}
+// 1 / 2^e, exact
+__device__ __forceinline__ float inverse_of(float scale) { return __uint_as_float((254u << 23) - __float_as_uint(scale)); }
+
+// Four numbers as e4m3, to the nearest, in a word.
+__device__ __forceinline__ unsigned pack4(float a, float b, float c, float d) {
+  auto in = [](float x) { return __builtin_amdgcn_fmed3f(x, -LARGEST, LARGEST); };
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(in(a), in(b), 0, false);
+  return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(in(c), in(d), r, true);
+}
+__device__ __forceinline__ unsigned rescale4(unsigned w, float by) {
+  const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  return pack4(a[0] * by, a[1] * by, b[0] * by, b[1] * by);
+}
+
+struct Pages {
+  uint8_t* k;
+  uint8_t* v;
+  float* ks;
+  float* vs;
+  int num_pages, KV, nb;  // nb: blocks of a page
+};
+__device__ __forceinline__ size_t block_index(const Pages& p, int page, int kvh, int sub) { return ((size_t)page * p.KV + kvh) * p.nb + sub; }
+
+// ---- appending ------------------------------------------------------------------------------------------
+//
+// One wave per (token, some query heads) and per (run of tokens of a block, kv head, keys or values).  A run: tokens next to each other in the
+// step that go to places next to each other of one block; its first token's wave does all of it, the others' leave.  A wave's lanes take a
+// token's head in pieces of four coordinates, 64 / LPT tokens (or query heads) at a time.
+template <int D> struct Lanes {
+  static constexpr int LPT = D <= 64 ? 16 : D <= 128 ? 32 : 64;  // lanes of a head, D / 4 of them busy
+  static constexpr int AT_ONCE = WAVE / LPT, PASSES = BLOCK / AT_ONCE;
+};
+
+template <int LPT> __device__ __forceinline__ float lanes_sum(float v) {
+  if constexpr (LPT == 64) v = plus_32(v);
+  if constexpr (LPT >= 32) v = plus_16(v);
+  v += dpp<DPP_ROTATE(8)>(v);
+  v += dpp<DPP_ROTATE(4)>(v);
+  v += dpp<DPP_XOR_2>(v);
+  return v + dpp<DPP_XOR_1>(v);
+}
+
+__device__ __forceinline__ void load4(const bf16* p, float (&x)[4]) {
+  const uint2 r = *reinterpret_cast<const uint2*>(p);
+  x[0] = __uint_as_float(r.x << 16); x[1] = __uint_as_float(r.x & 0xffff0000u);
+  x[2] = __uint_as_float(r.y << 16); x[3] = __uint_as_float(r.y & 0xffff0000u);
+}
+__device__ __forceinline__ void load4(const float* p, float (&x)[4]) {
+  const float4 r = *reinterpret_cast<const float4*>(p);
+  x[0] = r.x; x[1] = r.y; x[2] = r.z; x[3] = r.w;
+}
+
+struct Append {
+  const bf16* qkv;  // [T, H + 2 KV, D]
+  const void* qw;   // gains [D] of the per-head norms, or null
+  const void* kw;
+  const float2* cs;  // [T, R / 2] cos, sin, or null
+  const int* slots;  // [T]
+  bf16* q_out;       // [T, H, D]
+  Pages pages;
+  int T, H, R;
+  float eps;
+};
+
+// x: four coordinates of a head per lane; norm (w: gains) and rotation by the angles of token t.
+template <int D, typename W>
+__device__ __forceinline__ void norm_turn(float (&x)[4], const W* w, const float2* cs, float eps, int R, int t, int j) {
+  constexpr int LPT = Lanes<D>::LPT;
+  const bool busy = 4 * j < D;
+  if (w) {
+    const float ss = lanes_sum<LPT>(busy ? x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3] : 0.f);
+    const float inv = 1.0f / sqrtf(ss / (float)D + eps);
+    float g[4] = {0.f, 0.f, 0.f, 0.f};
+    if (busy) load4(w + 4 * j, g);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = x[i] * inv * g[i];
+  }
+  if (cs) {
+    const int half = R / 8;  // in pieces of four
+    const bool first = j < half, turns = j < 2 * half;
+    const int other = (threadIdx.x & (WAVE - 1)) + (first ? half : turns ? -half : 0);
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = __shfl(x[i], other, WAVE);
+    if (turns) {
+      const float4* angles = reinterpret_cast<const float4*>(cs + (size_t)t * (R / 2) + 4 * (first ? j : j - half));
+      const float4 a = angles[0], b = angles[1];
+      const float c[4] = {a.x, a.z, b.x, b.z}, s[4] = {a.y, a.w, b.y, b.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = first ? x[i] * c[i] - y[i] * s[i] : x[i] * c[i] + y[i] * s[i];
+    }
+  }
+}
+
+template <int D, typename W>
+__global__ __launch_bounds__(WAVE) void append8_kernel(Append a) {
+  constexpr int LPT = Lanes<D>::LPT, AT_ONCE = Lanes<D>::AT_ONCE, PASSES = Lanes<D>::PASSES;
+  __shared__ __align__(16) uint8_t turned[D * BLOCK];  // values of a run, transposed
+  const int t = blockIdx.x, lane = threadIdx.x, sub = lane / LPT, j = lane % LPT;
+  const int q_units = (a.H + AT_ONCE - 1) / AT_ONCE, KV = a.pages.KV, heads = a.H + 2 * KV;
+  const bool busy = 4 * j < D;
+  int unit = blockIdx.y;
+  if (unit < q_units) {
+    const int h = unit * AT_ONCE + sub;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (busy && h < a.H) load4(a.qkv + ((size_t)t * heads + h) * D + 4 * j, x);
+    norm_turn<D, W>(x, (const W*)a.qw, a.cs, a.eps, a.R, t, j);
+    if (busy && h < a.H) {
+      const bf16x4_t r = {(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]};
+      *reinterpret_cast<bf16x4_t*>(a.q_out + ((size_t)t * a.H + h) * D + 4 * j) = r;
+    }
+    return;
+  }
+  unit -= q_units;
+  const bool values = unit >= KV;
+  const int kvh = values ? unit - KV : unit;
+  const int slot = a.slots[t], bs = a.pages.nb * BLOCK;
+  if (slot < 0 || slot / bs >= a.pages.num_pages) return;
+  const int off = slot % BLOCK;
+  if (off > 0 && t > 0 && a.slots[t - 1] == slot - 1) return;  // an earlier token's run
+  const int most = min(BLOCK - off, a.T - t);
+  const bool goes_on = lane < most && a.slots[min(t + lane, a.T - 1)] == slot + lane;
+  const int n = __builtin_ctzll(~__ballot(goes_on));  // tokens of the run
+  const size_t block = block_index(a.pages, slot / bs, kvh, slot % bs / BLOCK);
+
+  float x[PASSES][4], amax = 0.f;
+  const bf16* src = a.qkv + ((size_t)t * heads + a.H + unit) * D + 4 * j;
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[p][i] = 0.f;
+    const int nth = p * AT_ONCE + sub;
+    if (busy && nth < n) load4(src + (size_t)nth * heads * D, x[p]);
+  }
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    if (!values && p * AT_ONCE < n)  // uniform
+      norm_turn<D, W>(x[p], (const W*)a.kw, a.cs, a.eps, a.R, t + min(p * AT_ONCE + sub, n - 1), j);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[p][i] = finite_or_zero(x[p][i]);
+      amax = fmaxf(amax, fabsf(x[p][i]));
+    }
+  }
+  amax = wave_max(amax);
+  float* scales = values ? a.pages.vs : a.pages.ks;
+  const float before = off > 0 ? scales[block] : 0.f;  // a block that begins with this run is new
+  const float scale = fmaxf(before, block_scale(amax)), inv = inverse_of(scale);
+  const bool grows = before > 0.f && scale > before;
+  const float by = before * inv;
+  uint8_t* at = (values ? a.pages.v : a.pages.k) + block * (BLOCK * D);
+  if (!values) {
+    if (grows) {  // the block's other rows at the new scale
+      for (int w = lane; w < BLOCK * D / 4; w += WAVE) {
+        const int row = 4 * w / D;
+        unsigned* word = reinterpret_cast<unsigned*>(at) + w;
+        if (row < off || row >= off + n) *word = rescale4(*word, by);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+      const int nth = p * AT_ONCE + sub;
+      if (busy && nth < n)
+        *reinterpret_cast<unsigned*>(at + (off + nth) * D + 4 * j) = pack4(x[p][0] * inv, x[p][1] * inv, x[p][2] * inv, x[p][3] * inv);
+    }
+  } else {
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+      const int nth = p * AT_ONCE + sub;
+      if (busy && nth < n) {
+        const unsigned w = pack4(x[p][0] * inv, x[p][1] * inv, x[p][2] * inv, x[p][3] * inv);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) turned[(4 * j + i) * BLOCK + off + nth] = (uint8_t)(w >> (8 * i));
+      }
+    }
+    __syncthreads();
+    // which bytes of a coordinate's 16 are the run's
+    u32x4_t mine;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      mine[w] = 0u;
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        if (4 * w + b >= off && 4 * w + b < off + n) mine[w] |= 0xffu << (8 * b);
+    }
+#pragma unroll
+    for (int d = lane; d < D; d += WAVE) {
+      u32x4_t* piece = reinterpret_cast<u32x4_t*>(at) + d;
+      u32x4_t out = *reinterpret_cast<const u32x4_t*>(turned + d * BLOCK);
+      if (n < BLOCK) {
+        u32x4_t held = *piece;
+        if (grows)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) held[w] = rescale4(held[w], by);
+        out = (out & mine) | (held & ~mine);
+      }
+      *piece = out;
+    }
+  }
+  if (lane == 0) scales[block] = scale;
+}
+
+// ---- attention --------------------------------------------------------------------------------------------
+//
+// A wave owns 16 columns, each a query of one head: the heads of a group for one token, or 16 queries of a prompt's tile.  It walks the keys in
+// steps of 64, four blocks, one of them each lane group's:
+//
+//   S^T[key][column] = K Q^T     the e4m3 keys as they are (16x16x128, 8-bit operands).  A query is scaled by a power of two as a block is and
+//                                split in two e4m3 parts, the number rounded and what is left of it: 4 + 4 bits hold a bf16 number's eight
+//                                exactly, down to 2^-10 of the query's largest coordinate, and what is smaller is off by 2^-19 of it at most.
+//   softmax                      fp32, base 2, maxima and sums kept per column
+//   O^T[d][column] += V^T P^T    values as bf16 (exact, the scale included), weights rounded to bf16
+//
+// Row r of score tile tt (0 .. 3) stands for key 16 (r / 4) + 4 tt + r % 4 of a step, so that the 16 keys whose weights a lane holds after the score
+// product are one block: one scale, and in the transposed values 16 bytes a coordinate.
+constexpr int STEP = 64;
+
+template <int D> struct Query {
+  u32x4_t high[D / 64], low[D / 64];  // coordinates 64 c + 16 grp .. + 15 of this lane's column
+  float scale;
+};
+
+template <int D> __device__ __forceinline__ void load_query(Query<D>& q, const bf16* row, int grp) {
+  float x[D / 64][16], amax = 0.f;
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      float four[4];
+      load4(row + 64 * c + 16 * grp + i, four);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        x[c][i + n] = four[n];
+        amax = fmaxf(amax, fabsf(four[n]));
+      }
+    }
+  q.scale = block_scale(quad_rows_max(amax));
+  const float inv = inverse_of(q.scale);
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      float y[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) y[n] = x[c][4 * w + n] * inv;
+      const unsigned high = pack4(y[0], y[1], y[2], y[3]);
+      const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)high, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)high, true);
+      q.high[c][w] = high;
+      q.low[c][w] = pack4(y[0] - a[0], y[1] - a[1], y[2] - b[0], y[3] - b[1]);
+    }
+}
+
+__device__ __forceinline__ i32x8_t both(u32x4_t a, u32x4_t b) {
+  return i32x8_t{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+}
+
+// scores of 16 keys, k: this lane's key, 16 bytes of every 64 coordinates
+template <int D> __device__ __forceinline__ f32x4_t score_tile(const u32x4_t (&k)[D / 64], const Query<D>& q) {
+  f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c + 1 < D / 64; c += 2) {
+    const i32x8_t kk = both(k[c], k[c + 1]);
+    s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kk, both(q.high[c], q.high[c + 1]), s, 0, 0, 0, 0, 0, 0);
+    s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kk, both(q.low[c], q.low[c + 1]), s, 0, 0, 0, 0, 0, 0);
+  }
+  if constexpr ((D / 64) % 2) {  // 64 coordinates that are left: both parts at once
+    constexpr int c = D / 64 - 1;
+    s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(both(k[c], k[c]), both(q.high[c], q.low[c]), s, 0, 0, 0, 0, 0, 0);
+  }
+  return s;
+}
+
+template <int D> struct Running {
+  f32x4_t o[D / 16];
+  float m, l;  // the column's maximum (base 2), and the sum of this lane's weights
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) o[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    m = NEG_INF;
+    l = 0.f;
+  }
+};
+
+// A request's pages as its block table names them; entries that are none of the pool's (of pages given back) are read as page 0, and keys beyond
+// `last` as those of its block: numbers, which masks hide.
+struct Table {
+  const int* entries;
+  int last;  // the last key that any column sees
+  __device__ __forceinline__ size_t block_of(const Pages& p, int key, int kvh) const {
+    const int n = min(key, last) / BLOCK, page = entries[n / p.nb];
+    return block_index(p, (unsigned)page < (unsigned)p.num_pages ? page : 0, kvh, n % p.nb);
+  }
+};
+
+// One step: the keys from kb on.  factor: from a score of e4m3 numbers to one in base 2 (natural units where scores are capped), without the block's scale.
+template <int D>
+__device__ __forceinline__ void step8(const Pages& pages, const Table& table, int kvh, int kb, const Query<D>& q, float factor, float cap, int pos,
+                                      int lo, int keep, Running<D>& run) {
+  const int lane = threadIdx.x & (WAVE - 1), col = lane & 15, grp = lane >> 4;
+  const size_t kblock = table.block_of(pages, kb + BLOCK * (col >> 2), kvh), vblock = table.block_of(pages, kb + BLOCK * grp, kvh);
+  f32x4_t s[4];
+  const uint8_t* krow = pages.k + kblock * (BLOCK * D) + (col & 3) * D + 16 * grp;
+#pragma unroll
+  for (int tt = 0; tt < 4; ++tt) {
+    u32x4_t k[D / 64];
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) k[c] = *reinterpret_cast<const u32x4_t*>(krow + 4 * tt * D + 64 * c);
+    s[tt] = score_tile<D>(k, q);
+  }
+  const float by = factor * pages.ks[vblock], vscale = pages.vs[vblock];
+  float mx = NEG_INF;
+#pragma unroll
+  for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float v = s[tt][r] * by;
+      if (cap > 0.f) v = cap * LOG2E * quick_tanh(v / cap);
+      const int key = kb + 16 * grp + 4 * tt + r;
+      s[tt][r] = key <= pos && (key >= lo || key < keep) ? v : NEG_INF;
+      mx = fmaxf(mx, s[tt][r]);
+    }
+  const float mn = fmaxf(run.m, quad_rows_max(mx)), base = mn == NEG_INF ? 0.f : mn;
+  const float alpha = __builtin_amdgcn_exp2f(run.m - base);
+  float sum = 0.f;
+  bf16x8_t p[2];
+#pragma unroll
+  for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float w = __builtin_amdgcn_exp2f(s[tt][r] - base);
+      sum += w;
+      p[tt >> 1][(tt & 1) * 4 + r] = (bf16)w;
+    }
+  run.m = mn;
+  run.l = run.l * alpha + sum;
+  const uint8_t* vcol = pages.v + vblock * (BLOCK * D) + BLOCK * col;
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d) {
+    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(vcol + 16 * BLOCK * d);
+    run.o[d] *= alpha;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      bf16x8_t vv;
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * h + w], vscale, false);
+        const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * h + w], vscale, true);
+        vv[4 * w] = a[0]; vv[4 * w + 1] = a[1]; vv[4 * w + 2] = b[0]; vv[4 * w + 3] = b[1];
+      }
+      run.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, p[h], run.o[d], 0, 0, 0);
+    }
+  }
+}
+
+// Which steps of 64 keys a walk takes: those from the sequence's start that hold kept tokens, then those from the first key in sight on.
+struct Steps {
+  int kept, base, count;
+  __device__ __forceinline__ Steps(int lo, int keep, int last) {  // lo: the first key of any column's window; last: the last key
+    const int k = min(keep, lo);
+    kept = (k + STEP - 1) / STEP;
+    base = lo / STEP;
+    if (kept > 0 && kept >= base) kept = base = 0;
+    count = last < 0 ? 0 : kept + last / STEP - base + 1;
+  }
+  __device__ __forceinline__ int first_key(int at) const { return STEP * (at < kept ? at : at - kept + base); }
+};
+
+struct Attend {
+  const bf16* q;
+  Pages pages;
+  const int* items;      // single queries: the tokens, or null for all
+  const int* positions;
+  const int* tok_row;    // null: token t is row t
+  const int* tiles;      // portions: [num_tiles, 4] first token, count, row, first position
+  const int* tables;
+  int table_width;
+  bf16* out;
+  float *part_m, *part_l, *part_acc;
+  int H, KV, share;      // KV: groups of query heads; `share` of them read one head of the pages
+  float scale;
+  Sight sight;
+  int part_steps, P;
+};
+
+__device__ __forceinline__ float score_factor(const Attend& a) { return a.sight.cap > 0.f ? a.scale : a.scale * LOG2E; }
+
+// The weighted sum over its denominator; nothing seen: 0.  m in base 2.
+__device__ __forceinline__ float share_of(const Sight& sight, int head, float m, float l) {
+  if (sight.sink) {
+    const float sk = sink_score(1, sight.sinks, head) * LOG2E, top = fmaxf(m, sk), e = __builtin_amdgcn_exp2f(m - top);
+    return e / (l * e + __builtin_amdgcn_exp2f(sk - top));
+  }
+  return l > 0.f ? 1.0f / l : 0.f;
+}
+
+// One workgroup per (token, group of query heads, partition of its keys); its four waves take the steps in turn.
+template <int D>
+__global__ __launch_bounds__(256) void single8_kernel(Attend a) {
+  constexpr int LD = D + 4;
+  extern __shared__ __align__(16) float smem[];  // [4][16] m, [4][16] l, [4][G][LD]
+  const int G = a.H / a.KV, item = blockIdx.x, kvh = blockIdx.y, part = blockIdx.z, h0 = kvh * G;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, grp = lane >> 4;
+  const int t = a.items ? a.items[item] : item, bs = a.pages.nb * BLOCK;
+  const int pos = min(a.positions[t], a.table_width * bs - 1);
+  const int lo = first_in_window(a.sight, pos + 1);
+  const Table table{a.tables + (size_t)(a.tok_row ? a.tok_row[t] : t) * a.table_width, pos};
+  const Steps steps(lo, a.sight.keep, pos);
+  const int from = part * a.part_steps, to = min(steps.count, from + a.part_steps);
+  Running<D> run;
+  run.clear();
+  Query<D> q;
+  load_query<D>(q, a.q + ((size_t)t * a.H + h0 + min(col, G - 1)) * D, grp);
+  const float factor = score_factor(a) * q.scale;
+  for (int at = from + wave; at < to; at += 4)
+    step8<D>(a.pages, table, kvh / a.share, steps.first_key(at), q, factor, a.sight.cap, pos, lo, a.sight.keep, run);
+  run.l = quad_rows_sum(run.l);
+  float *sm = smem, *sl = smem + 64, *so = smem + 128;
+  if (grp == 0 && col < G) { sm[wave * 16 + col] = run.m; sl[wave * 16 + col] = run.l; }
+  if (col < G)
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f32x4_t*>(so + (wave * G + col) * LD + d * 16 + 4 * grp) = run.o[d];
+  __syncthreads();
+  for (int i = tid; i < G * D; i += 256) {
+    const int g = i / D, d = i % D, h = h0 + g;
+    float m = NEG_INF, num = 0.f, den = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) m = fmaxf(m, sm[w * 16 + g]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float e = m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(sm[w * 16 + g] - m);
+      num += so[(w * G + g) * LD + d] * e;
+      den += sl[w * 16 + g] * e;
+    }
+    if (a.P == 1) {
+      put(a.out, ((size_t)t * a.H + h) * D + d, num * share_of(a.sight, h, m, den), a.sight.wide);
+    } else {
+      const size_t o = ((size_t)item * a.H + h) * a.P + part;
+      a.part_acc[o * D + d] = num;
+      if (d == 0) { a.part_m[o] = m; a.part_l[o] = den; }
+    }
+  }
+}
+
+// The partitions of every (token, head): sum acc_p 2^(m_p - m) / sum l_p 2^(m_p - m).
+__global__ __launch_bounds__(256) void single8_merge_kernel(Attend a, int D) {
+  const int item = blockIdx.x, h = blockIdx.y, t = a.items ? a.items[item] : item;
+  const size_t base = ((size_t)item * a.H + h) * a.P;
+  float m = NEG_INF;
+  for (int p = 0; p < a.P; ++p) m = fmaxf(m, a.part_m[base + p]);
+  for (int d = threadIdx.x; d < D; d += blockDim.x) {
+    float num = 0.f, den = 0.f;
+    for (int p = 0; p < a.P; ++p) {
+      const float e = m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(a.part_m[base + p] - m);
+      num += a.part_acc[(base + p) * D + d] * e;
+      den += a.part_l[base + p] * e;
+    }
+    put(a.out, ((size_t)t * a.H + h) * D + d, num * share_of(a.sight, h, m, den), a.sight.wide);
+  }
+}
+
+// Portions of prompts: one workgroup per (tile of up to 64 queries, query head), a wave 16 of its queries.
+template <int D>
+__global__ __launch_bounds__(256) void prompt8_kernel(Attend a) {
+  const int tile = blockIdx.x, head = blockIdx.y, kvh = head / (a.H / a.KV);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, grp = lane >> 4;
+  const int tok0 = a.tiles[4 * tile], count = a.tiles[4 * tile + 1], pos0 = a.tiles[4 * tile + 3], bs = a.pages.nb * BLOCK;
+  const int q0 = 16 * wave, n = min(16, count - q0);
+  if (n <= 0) return;
+  const int mine = min(col, n - 1), t = tok0 + q0 + mine, end = a.table_width * bs - 1;
+  const int pos = min(pos0 + q0 + mine, end), last = min(pos0 + q0 + n - 1, end);
+  const int lo = first_in_window(a.sight, pos + 1), first = first_in_window(a.sight, pos0 + q0 + 1);
+  const Table table{a.tables + (size_t)a.tiles[4 * tile + 2] * a.table_width, last};
+  const Steps steps(first, a.sight.keep, last);
+  Running<D> run;
+  run.clear();
+  Query<D> q;
+  load_query<D>(q, a.q + ((size_t)t * a.H + head) * D, grp);
+  const float factor = score_factor(a) * q.scale;
+  for (int at = 0; at < steps.count; ++at)
+    step8<D>(a.pages, table, kvh, steps.first_key(at), q, factor, a.sight.cap, pos, lo, a.sight.keep, run);
+  const float inv = share_of(a.sight, head, run.m, quad_rows_sum(run.l));
+  if (col >= n) return;
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) put(a.out, ((size_t)t * a.H + head) * D + 16 * d + 4 * grp + r, run.o[d][r] * inv, a.sight.wide);
+}
+
+bool pages_ok(const void* k, const void* v, const float* ks, const float* vs, int num_pages, int KV, int D, int bs) {
+  return k && v && ks && vs && num_pages > 0 && KV > 0 && D > 0 && D % 64 == 0 && D <= 256 && bs > 0 && bs % BLOCK == 0 &&
+         !(((uintptr_t)k | (uintptr_t)v) & 15);
+}
+Pages pages_of(const void* k, const void* v, const float* ks, const float* vs, int num_pages, int KV, int bs) {
+  return Pages{(uint8_t*)k, (uint8_t*)v, (float*)ks, (float*)vs, num_pages, KV, bs / BLOCK};
+}
+
+}  // namespace
+
+#define FOR_WIDTH(CALL)       \
+  switch (D / 64) {           \
+    case 1: CALL(64); break;  \
+    case 2: CALL(128); break; \
+    case 3: CALL(192); break; \
+    default: CALL(256); break; \
+  }
+
+// Per-head norm (qw, kw: gains [D], or null), rotation of the first R coordinates in pairs (i, i + R/2) (cs [T, R/2] cos, sin, or null),
+// queries to q_out [T, H, D] and, with store, keys and values into the blocks that `slots` name (page * bs + offset; none for a negative one).
+// qkv [T, H + 2 KV, D] bf16; D a multiple of 64 up to 256, R of 8, bs of 16.  Tokens of one block come as one run: next to each other, in the
+// order of their places; a run that starts at a block's first place makes it new.
+extern "C" int as_qk_norm_rope_store8(const void* qkv, const void* qw, const void* kw, int w_dtype, const float* cs, const int* slots,
+                                      void* q_out, void* k_pages, void* v_pages, float* k_scales, float* v_scales, int num_pages, int num_tokens,
+                                      int H, int KV, int D, int R, float eps, int bs, int store, hipStream_t stream) {
+  if (num_tokens <= 0) return AS_OK;
+  if (H <= 0 || KV <= 0 || D <= 0 || D % 64 || D > 256 || R < 0 || R > D || R % 8 || (R > 0) != (cs != nullptr)) return AS_BAD_SHAPE;
+  if ((qw == nullptr) != (kw == nullptr) || !qkv || !q_out) return AS_BAD_SHAPE;
+  if (store && (!slots || !pages_ok(k_pages, v_pages, k_scales, v_scales, num_pages, KV, D, bs))) return AS_BAD_SHAPE;
+  if (w_dtype != DT_F32 && w_dtype != DT_BF16) return AS_BAD_DTYPE;
+  const Append a{(const bf16*)qkv, qw, kw, (const float2*)cs, slots, (bf16*)q_out,
+                 pages_of(k_pages, v_pages, k_scales, v_scales, num_pages, KV, bs), num_tokens, H, R, eps};
+#define LAUNCH(DV)                                                                          \
+  {                                                                                         \
+    constexpr int at_once = Lanes<DV>::AT_ONCE;                                             \
+    const dim3 grid(num_tokens, (H + at_once - 1) / at_once + (store ? 2 * KV : 0));        \
+    if (w_dtype == DT_F32) append8_kernel<DV, float><<<grid, WAVE, 0, stream>>>(a);         \
+    else append8_kernel<DV, bf16><<<grid, WAVE, 0, stream>>>(a);                            \
+  }
+  FOR_WIDTH(LAUNCH)
+#undef LAUNCH
+  return launch_status();
+}
+
+// Single queries.  part_m, part_l [N, H, P], part_acc [N, H, P, D] fp32 where P > 1; part_size: keys of a partition, a multiple of 64; share: how
+// many of the KV groups of query heads (at most 16 to a group) read one head of the pages, which hold KV / share.
+extern "C" int as_attn_single_query8(const void* q, const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
+                                     int num_pages, const int* items, int num_items, const int* positions, const int* tok_row,
+                                     const int* block_tables, int table_width, void* out, float* part_m, float* part_l, float* part_acc, int H,
+                                     int KV, int D, int bs, float scale, int window, int keep, int chunk, float cap, int sink,
+                                     const float* sinks, int wide, int part_size, int P, int share, hipStream_t stream) {
+  if (num_items <= 0) return AS_OK;
+  const Sight sight{window, keep, chunk, cap, sink, sinks, wide};
+  if (!sight_ok(sight) || H <= 0 || KV <= 0 || H % KV || H / KV > 16 || share < 1 || KV % share) return AS_BAD_SHAPE;
+  if (!pages_ok(k_pages, v_pages, k_scales, v_scales, num_pages, KV / share, D, bs) || table_width <= 0) return AS_BAD_SHAPE;
+  if (!q || !positions || !block_tables || !out || part_size <= 0 || part_size % STEP || P <= 0 || P > 65535) return AS_BAD_SHAPE;
+  if (P > 1 && (!part_m || !part_l || !part_acc)) return AS_BAD_SHAPE;
+  const Attend a{(const bf16*)q, pages_of(k_pages, v_pages, k_scales, v_scales, num_pages, KV / share, bs), items, positions, tok_row, nullptr,
+                 block_tables, table_width, (bf16*)out, part_m, part_l, part_acc, H, KV, share, scale, sight, part_size / STEP, P};
+  const size_t shmem = sizeof(float) * (128 + 4 * (size_t)(D + 4) * (H / KV));
+#define LAUNCH(DV)                                                                                                                       \
+  {                                                                                                                                      \
+    const auto kernel = single8_kernel<DV>;                                                                                              \
+    if (shmem > 65536 && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)shmem) != hipSuccess) \
+      return AS_LAUNCH_FAILED;                                                                                                           \
+    kernel<<<dim3(num_items, KV, P), 256, shmem, stream>>>(a);                                                                           \
+  }
+  FOR_WIDTH(LAUNCH)
+#undef LAUNCH
+  if (hipGetLastError() != hipSuccess) return AS_LAUNCH_FAILED;
+  if (P > 1) single8_merge_kernel<<<dim3(num_items, H), D <= 64 ? 64 : D <= 128 ? 128 : 256, 0, stream>>>(a, D);
+  return launch_status();
+}
+
+// Portions of prompts: tiles [num_tiles, 4] int32 (first token, count <= 64, row of block_tables, position of the first).
+extern "C" int as_attn_prefill8(const void* q, const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
+                                int num_pages, const int* tiles, int num_tiles, const int* block_tables, int table_width, void* out, int H,
+                                int KV, int D, int bs, float scale, int window, int keep, int chunk, float cap, int sink, const float* sinks,
+                                int wide, hipStream_t stream) {
+  if (num_tiles <= 0) return AS_OK;
+  const Sight sight{window, keep, chunk, cap, sink, sinks, wide};
+  if (!sight_ok(sight) || H <= 0 || KV <= 0 || H % KV || H > 65535) return AS_BAD_SHAPE;
+  if (!pages_ok(k_pages, v_pages, k_scales, v_scales, num_pages, KV, D, bs) || table_width <= 0) return AS_BAD_SHAPE;
+  if (!q || !tiles || !block_tables || !out) return AS_BAD_SHAPE;
+  const Attend a{(const bf16*)q, pages_of(k_pages, v_pages, k_scales, v_scales, num_pages, KV, bs), nullptr, nullptr, nullptr, tiles, block_tables,
+                 table_width, (bf16*)out, nullptr, nullptr, nullptr, H, KV, 1, scale, sight, 0, 1};
+#define LAUNCH(DV) prompt8_kernel<DV><<<dim3(num_tiles, H), 256, 0, stream>>>(a)
+  FOR_WIDTH(LAUNCH)
+#undef LAUNCH
+  return launch_status();
+}

@@ -21,7 +21,7 @@ ARCH = "gfx950"
 FLAGS = ["-O3", "-std=c++17", "-shared", "-fPIC", f"--offload-arch={ARCH}",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wno-unused-command-line-argument"]  # fmt: skip
 HEADERS = ["attn_parts.h", "common.h", "float_parts.h", "no_alloc.h", "rows.h", "wide_tile.h"]
-LIBRARIES = ("elementwise", "attention", "attention_mix", "gemm", "gemm_wide", "gemm_f32", "sampling", "blas", "recurrent", "moe", "layer_ops",
+LIBRARIES = ("elementwise", "attention", "attention_mix", "cache8", "gemm", "gemm_wide", "gemm_f32", "sampling", "blas", "recurrent", "moe", "layer_ops",
              "linear_attention", "latent", "streams", "sandwich", "state_space", "launches")
 LINK = {"blas": ["-lhipblaslt"]}  # what a library links beside the HIP runtime
 

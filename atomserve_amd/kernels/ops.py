@@ -783,6 +783,154 @@ def attn_mixed(q, k_pages, v_pages, items, tiles, positions, tok_row, block_tabl
          part_size, P, _stream())  # fmt: skip
 
 
+# ---- a cache in 8 bits -------------------------------------------------------------------------------
+#
+# Keys and values as e4m3 numbers in blocks of 16 tokens; for every block and kv head one scale for the keys and one for the values: the power of
+# two 2^e with the smallest e in -100 .. 119 for which the block's largest magnitude is at most 448 * 2^e.  Half of a bfloat16 cache's bytes: twice
+# the tokens in the same memory, and half of what the attention of single queries waits for.  A number is off by at most 2^-4 of itself.
+#
+#   k_pages  [num_pages, KV, block_size, D]             float8_e4m3fn
+#   v_pages  [num_pages, KV, block_size / 16, D, 16]    float8_e4m3fn (a block's values are transposed)
+#   k_scales, v_scales  [num_pages, KV, block_size / 16]  fp32
+#
+# Slots and block tables are those of a 16-bit cache.  What a block holds is known once its first place is written: a call that writes the first place
+# makes the block new and forgets what it held, and a call that goes on in a block lets its scale grow and rewrites it.  Pools start zeroed.
+
+E4M3 = torch.float8_e4m3fn
+BLOCK8 = 16  # tokens that share a scale
+STEP8 = 64  # keys that a wave of the attention kernels takes at a time
+
+
+def cache8_supported(dtype, num_heads: int, num_kv_heads: int, head_dim: int, block_size: int, rotary_dim: int = 0) -> bool:
+    """Whether the cache in 8 bits takes these heads: bfloat16 heads of 64, 128, 192 or 256, rotated in a multiple of 8 coordinates, pages of a
+    multiple of 16 tokens."""
+    return (dtype == BF16 and head_dim % 64 == 0 and 0 < head_dim <= 256 and num_heads % num_kv_heads == 0 and block_size % BLOCK8 == 0
+            and rotary_dim % 8 == 0)  # fmt: skip
+
+
+def _check_pages8(k_pages, v_pages, k_scales, v_scales, num_kv_heads=None) -> tuple:
+    """(pages, kv heads, tokens of a page, head width) of a cache in 8 bits."""
+    _check(k_pages, "k_pages", E4M3, (None, num_kv_heads, None, None))
+    NB, KV, bs, D = k_pages.shape
+    if bs % BLOCK8 or bs == 0 or D % 64 or not 0 < D <= 256 or NB == 0 or KV == 0:
+        raise KernelError(f"a cache in 8 bits has pages of a multiple of {BLOCK8} tokens and heads of 64, 128, 192 or 256, not {bs} and {D}")
+    _check(v_pages, "v_pages", E4M3, (NB, KV, bs // BLOCK8, D, BLOCK8))
+    _check(k_scales, "k_scales", F32, (NB, KV, bs // BLOCK8))
+    _check(v_scales, "v_scales", F32, (NB, KV, bs // BLOCK8))
+    return NB, KV, bs, D
+
+
+def qk_norm_rope_store8(qkv, q_weight, k_weight, cos_sin, slots, q_out, k_pages, v_pages, k_scales, v_scales, num_heads, num_kv_heads, eps,
+                        store_kv=True) -> None:  # fmt: skip
+    """`qk_norm_rope_store` into a cache in 8 bits: per-head norm (if weights are given) and rotation (if `cos_sin` is given, of a
+    multiple of 8 coordinates), queries to q_out, keys and values, rounded once from 32 bits, into the blocks that `slots` name.
+
+    qkv [T, H + 2 KV, D], q_out [T, H, D] bfloat16; slots [T] int32 (page * block_size + offset, or -1 for a token whose keys are not stored; one
+    beyond the pages stores nothing either).  The tokens that go into one block come as one run, next to each other and in the order of their places, as a request's
+    tokens do: two runs of one call in one block, or one place twice, leave that block undefined.  What is not finite is stored as zero."""
+    _check(qkv, "qkv", BF16, (None, num_heads + 2 * num_kv_heads, None))
+    T, _, D = qkv.shape
+    _check(q_out, "q_out", BF16, (T, num_heads, D))
+    R = 0
+    if cos_sin is not None:
+        _check(cos_sin, "cos_sin", F32, (T, None, 2))
+        R = 2 * cos_sin.shape[1]
+    if R > D or R % 8 or D % 64 or not 0 < D <= 256:
+        raise KernelError(f"appending in 8 bits: unsupported head width {D} (64, 128, 192 or 256) or rotary width {R} (a multiple of 8)")
+    if (q_weight is None) != (k_weight is None):
+        raise KernelError("q and k norm weights come together")
+    w_dtype = BF16
+    if q_weight is not None:
+        _check(q_weight, "q_weight", (F32, BF16), (D,))
+        _check(k_weight, "k_weight", q_weight.dtype, (D,))
+        w_dtype = q_weight.dtype
+    NB, bs = 1, BLOCK8
+    if store_kv:
+        _check(slots, "slots", I32, (T,))
+        NB, _, bs, width = _check_pages8(k_pages, v_pages, k_scales, v_scales, num_kv_heads)
+        if width != D:
+            raise KernelError(f"k_pages has heads of {width}, qkv of {D}")
+    held = (_ptr(slots), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales)) if store_kv else (0,) * 5
+    call("as_qk_norm_rope_store8", _ptr(qkv), _ptr(q_weight), _ptr(k_weight), _DT[w_dtype], _ptr(cos_sin) if R else 0, held[0], _ptr(q_out),
+         *held[1:], NB, T, num_heads, num_kv_heads, D, R, float(eps), bs, int(bool(store_kv)), _stream())  # fmt: skip
+
+
+def _up64(n: int) -> int:
+    return -(-n // STEP8) * STEP8
+
+
+def _partitions8(N, H, KV, D, max_context, window, part_size, device, keep_first=0):
+    """`_partitions` for the kernel of single queries over 8 bits, whose steps are 64 keys."""
+    span = _up64(max_context) if window <= 0 else min(_up64(max_context), _up64(window + STEP8 - 1) + _up64(keep_first))
+    if part_size is None:
+        if N * KV >= attn_fill_groups():
+            part_size = span
+        else:
+            part_size = min(MFMA_PARTITIONS, key=lambda part: _partition_cost(N * KV, span, part) + (MERGE_LAUNCH if part < span else 0.0))
+    if part_size <= 0 or part_size % STEP8:
+        raise KernelError(f"attention over 8 bits: partitions are multiples of {STEP8} keys")
+    P = max(1, math.ceil(span / part_size))
+    part_m = part_l = part_acc = None
+    if P > 1:
+        part_m = torch.empty((N, H, P), dtype=F32, device=device)
+        part_l = torch.empty((N, H, P), dtype=F32, device=device)
+        part_acc = torch.empty((N, H, P, D), dtype=F32, device=device)
+    return part_size, P, part_m, part_l, part_acc
+
+
+def _share8(group: int) -> int:
+    """Into how many equal groups of at most 16 the query heads of a kv head are cut."""
+    return next(n for n in range(1, group + 1) if group % n == 0 and group // n <= 16)
+
+
+def attn_single_query8(q, k_pages, v_pages, k_scales, v_scales, items, positions, tok_row, block_tables, out, scale, window, max_context,
+                       part_size=None, keep_first=0, softcap=0.0, sink=False, chunk=0) -> None:  # fmt: skip
+    """`attn_single_query` of bfloat16 heads over a cache in 8 bits: arguments as there.  A query at a negative position sees nothing: zeros."""
+    _check(q, "q", BF16, (None, None, None))
+    T, H, D = q.shape
+    sight = _sight(window, keep_first, chunk, softcap, sink, q, out)
+    NB, KV, bs, width = _check_pages8(k_pages, v_pages, k_scales, v_scales)
+    if items is not None:
+        _check(items, "items", I32, (None,))
+    _check(positions, "positions", I32, (T,))
+    if tok_row is not None:
+        _check(tok_row, "tok_row", I32, (T,))
+    _check(block_tables, "block_tables", I32, (None, None))
+    if tok_row is None and block_tables.shape[0] < T:
+        raise KernelError(f"attention: {T} tokens that are their own rows need as many block tables")
+    N = T if items is None else items.shape[0]
+    if N == 0:
+        return
+    if H % KV or width != D:
+        raise KernelError(f"attention over 8 bits: heads {H}/{KV} of {D} do not fit pages of heads of {width}")
+    if max_context > block_tables.shape[1] * bs:
+        raise KernelError("attention: block tables are shorter than the longest context")
+    share = _share8(H // KV)
+    part_size, P, part_m, part_l, part_acc = _partitions8(N, H, KV * share, D, max_context, window or chunk, part_size, q.device, sight[1])
+    call("as_attn_single_query8", _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales), NB, _ptr(items), N, _ptr(positions),
+         _ptr(tok_row), _ptr(block_tables), block_tables.shape[1], _ptr(out), _ptr(part_m), _ptr(part_l), _ptr(part_acc), H, KV * share, D, bs,
+         float(scale), *sight, part_size, P, share, _stream())  # fmt: skip
+
+
+def attn_prefill8(q, k_pages, v_pages, k_scales, v_scales, tiles, block_tables, out, scale, window, max_context, tile_keys: int = 0, keep_first=0,
+                  softcap=0.0, sink=False, chunk=0) -> None:  # fmt: skip
+    """`attn_prefill` over a cache in 8 bits: arguments as there."""
+    _check(q, "q", BF16, (None, None, None))
+    T, H, D = q.shape
+    sight = _sight(window, keep_first, chunk, softcap, sink, q, out)
+    NB, KV, bs, width = _check_pages8(k_pages, v_pages, k_scales, v_scales)
+    _check(tiles, "tiles", I32, (None, 4))
+    _check(block_tables, "block_tables", I32, (None, None))
+    if tiles.shape[0] == 0:
+        return
+    if H % KV or width != D:
+        raise KernelError(f"prefill attention over 8 bits: heads {H}/{KV} of {D} do not fit pages of heads of {width}")
+    if max_context > block_tables.shape[1] * bs:
+        raise KernelError("attention: block tables are shorter than the longest context")
+    call("as_attn_prefill8", _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales), NB, _ptr(tiles), tiles.shape[0],
+         _ptr(block_tables), block_tables.shape[1], _ptr(out), H, KV, D, bs, float(scale), *sight, _stream())  # fmt: skip
+
+
 SKINNY_MAX_ROWS = 16  # up to here the bf16 product streams the weights through our own kernel
 # 17 to 32 rows: the persistent kernel keeps two row tiles in registers up to this K ...
 SKINNY_TWO_MAX_ROWS, SKINNY_TWO_MAX_K = 32, 4096

@@ -1,0 +1,126 @@
+"""The cache in 8 bits where no GPU is needed: what its calls refuse, before anything is launched."""
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from atomserve_amd.kernels import ops
+
+BF16, F32, I32, E4M3 = torch.bfloat16, torch.float32, torch.int32, torch.float8_e4m3fn
+
+
+@pytest.fixture(autouse=True)
+def nothing_is_launched(monkeypatch):
+    def call(name, *args):
+        raise AssertionError(f"{name} would have been launched")
+
+    monkeypatch.setattr(ops, "call", call)
+    monkeypatch.setattr(ops, "_ptr", lambda t: 0)
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(ops, "_compute_units", 256)
+    with FakeTensorMode():  # tensors that say they are on the GPU, without memory
+        yield
+
+
+def tensor(*shape, dtype=BF16):
+    return torch.empty(shape, dtype=dtype, device="cuda:0")
+
+
+def cache(KV=2, bs=16, D=64, NB=4, **kw):
+    made = {"k_pages": tensor(NB, KV, bs, D, dtype=E4M3), "v_pages": tensor(NB, KV, bs // 16, D, 16, dtype=E4M3),
+            "k_scales": tensor(NB, KV, bs // 16, dtype=F32), "v_scales": tensor(NB, KV, bs // 16, dtype=F32)}  # fmt: skip
+    return {**made, **kw}
+
+
+def append(T=3, H=4, KV=2, D=64, **kw):
+    args = {"qkv": tensor(T, H + 2 * KV, D), "q_weight": None, "k_weight": None, "cos_sin": tensor(T, D // 2, 2, dtype=F32),
+            "slots": tensor(T, dtype=I32), "q_out": tensor(T, H, D), **cache(KV, D=D), "num_heads": H, "num_kv_heads": KV, "eps": 1e-6}  # fmt: skip
+    ops.qk_norm_rope_store8(**{**args, **kw})
+
+
+def single(T=3, H=4, KV=2, D=64, **kw):
+    args = {"q": tensor(T, H, D), **cache(KV, D=D), "items": None, "positions": tensor(T, dtype=I32), "tok_row": None,
+            "block_tables": tensor(T, 4, dtype=I32), "out": tensor(T, H, D), "scale": 0.1, "window": 0, "max_context": 64}  # fmt: skip
+    ops.attn_single_query8(**{**args, **kw})
+
+
+def prompt(T=70, H=4, KV=2, D=64, **kw):
+    args = {"q": tensor(T, H, D), **cache(KV, D=D), "tiles": tensor(2, 4, dtype=I32), "block_tables": tensor(1, 8, dtype=I32),
+            "out": tensor(T, H, D), "scale": 0.1, "window": 0, "max_context": 70}  # fmt: skip
+    ops.attn_prefill8(**{**args, **kw})
+
+
+@pytest.mark.parametrize("call", [append, single, prompt])
+def test_what_fits_goes_to_the_kernel(call):
+    with pytest.raises(AssertionError, match="would have been launched"):
+        call()
+
+
+@pytest.mark.parametrize("call", [append, single, prompt])
+@pytest.mark.parametrize("wrong", [
+    {"k_pages": lambda: tensor(4, 2, 16, 64, dtype=BF16)},  # not 8 bits
+    {"v_pages": lambda: tensor(4, 2, 64, 16, dtype=E4M3)},  # the layout of a 16-bit cache
+    {"v_pages": lambda: tensor(3, 2, 1, 64, 16, dtype=E4M3)},  # fewer pages
+    {"k_scales": lambda: tensor(4, 2, 1, dtype=BF16)},
+    {"k_scales": lambda: tensor(4, 2, dtype=F32)},
+    {"v_scales": lambda: tensor(4, 2, 2, dtype=F32)},
+    {"v_scales": lambda: torch.empty(4, 2, 1)},  # on the host
+    {"k_pages": lambda: tensor(4, 2, 64, 16, dtype=E4M3).transpose(2, 3)},  # strides
+])  # fmt: skip
+def test_pages_that_do_not_fit_are_refused(call, wrong):
+    with pytest.raises(ops.KernelError):
+        call(**{k: v() for k, v in wrong.items()})
+
+
+@pytest.mark.parametrize("call", [append, single, prompt])
+@pytest.mark.parametrize("D,bs", [(32, 16), (96, 16), (320, 16), (64, 24), (64, 8)])
+def test_heads_and_pages_that_no_kernel_takes_are_refused(call, D, bs):
+    with pytest.raises(ops.KernelError):
+        call(D=D, **cache(D=D, bs=max(16, bs // 16 * 16), k_pages=tensor(4, 2, bs, D, dtype=E4M3)))
+
+
+@pytest.mark.parametrize("wrong", [
+    {"qkv": lambda: tensor(3, 8, 64, dtype=F32)}, {"qkv": lambda: tensor(3, 7, 64)}, {"q_out": lambda: tensor(3, 4, 64, dtype=F32)},
+    {"slots": lambda: tensor(4, dtype=I32)}, {"slots": lambda: tensor(3, dtype=torch.int64)}, {"cos_sin": lambda: tensor(3, 34, 2, dtype=F32)},
+    {"cos_sin": lambda: tensor(3, 33, 2, dtype=F32)}, {"cos_sin": lambda: tensor(3, 2, 2, dtype=F32)[:, :1].contiguous()},
+    {"cos_sin": lambda: tensor(2, 32, 2, dtype=F32)}, {"q_weight": lambda: tensor(64)}, {"k_weight": lambda: tensor(64)},
+    {"q_weight": lambda: tensor(64), "k_weight": lambda: tensor(64, dtype=F32)}, {"q_weight": lambda: tensor(32), "k_weight": lambda: tensor(32)},
+])  # fmt: skip
+def test_appending_refuses(wrong):
+    with pytest.raises(ops.KernelError):
+        append(**{k: v() for k, v in wrong.items()})
+
+
+@pytest.mark.parametrize("wrong", [
+    {"q": lambda: tensor(3, 4, 64, dtype=F32)}, {"q": lambda: tensor(3, 3, 64), "out": lambda: tensor(3, 3, 64)}, {"out": lambda: tensor(3, 4, 32)},
+    {"q": lambda: tensor(3, 4, 128), "out": lambda: tensor(3, 4, 128)}, {"positions": lambda: tensor(2, dtype=I32)},
+    {"block_tables": lambda: tensor(2, 4, dtype=I32)}, {"max_context": lambda: 65}, {"window": lambda: -1}, {"softcap": lambda: -1.0},
+    {"window": lambda: 5, "chunk": lambda: 5}, {"part_size": lambda: 32}, {"part_size": lambda: 96}, {"part_size": lambda: 0},
+    {"sink": lambda: tensor(3, dtype=F32)}, {"items": lambda: tensor(2, dtype=torch.int64)}, {"tok_row": lambda: tensor(2, dtype=I32)},
+])  # fmt: skip
+def test_single_queries_refuse(wrong):
+    with pytest.raises(ops.KernelError):
+        single(**{k: v() for k, v in wrong.items()})
+
+
+@pytest.mark.parametrize("wrong", [
+    {"q": lambda: tensor(70, 4, 64, dtype=F32)}, {"q": lambda: tensor(70, 5, 64), "out": lambda: tensor(70, 5, 64)},
+    {"tiles": lambda: tensor(2, 3, dtype=I32)}, {"tiles": lambda: tensor(2, 4, dtype=torch.int64)}, {"max_context": lambda: 129},
+    {"keep_first": lambda: -1}, {"q": lambda: tensor(70, 4, 128), "out": lambda: tensor(70, 4, 128)},
+])  # fmt: skip
+def test_prompts_refuse(wrong):
+    with pytest.raises(ops.KernelError):
+        prompt(**{k: v() for k, v in wrong.items()})
+
+
+def test_nothing_to_do_launches_nothing():
+    single(items=tensor(0, dtype=I32))
+    prompt(tiles=tensor(0, 4, dtype=I32))
+
+
+def test_which_heads_the_cache_takes():
+    takes = ops.cache8_supported
+    assert takes(BF16, 32, 8, 128, 16, 128) and takes(BF16, 24, 1, 256, 48, 0) and takes(BF16, 28, 4, 64, 64, 8)
+    assert not takes(F32, 32, 8, 128, 16) and not takes(BF16, 32, 8, 96, 16) and not takes(BF16, 32, 8, 128, 8) and not takes(BF16, 9, 2, 128, 16)
+    assert not takes(BF16, 32, 8, 128, 16, 12) and not takes(BF16, 8, 8, 320, 16)
+    assert [ops._share8(g) for g in (1, 7, 16, 17, 24, 32, 40)] == [1, 1, 1, 17, 2, 2, 4]
