@@ -312,6 +312,128 @@ template <int D> struct Running {
   }
 };
 
+// The blocks of a step's keys as a request's table names them.  Keys are uniform over the wave and its scalar unit finds them: the division by a page's
+// blocks is a product with `magic` = ceil(2^32 / blocks), exact while 16-token blocks of a context times blocks of a page stay under 2^32.
+// Entries that are none of the pool's (of pages given back) are read as page 0, and keys beyond the last as those of its block: numbers, which masks hide.
+struct Pieces {
+  const int* entries;
+  int last;  // the last block that a query sees
+  unsigned magic;
+};
+struct Blocks {  // pages as the table has them, and blocks within a page; asked for here, looked at a step later
+  unsigned p0, p1, p2, p3, s0, s1, s2, s3;
+  static __device__ __forceinline__ void ask(const Pages& pages, const Pieces& pieces, int key, unsigned& page, unsigned& sub) {
+    const unsigned n = min(key / BLOCK, pieces.last), entry = __umulhi(n, pieces.magic) + n * (pages.nb == 1);
+    page = pieces.entries[entry];
+    sub = n - entry * pages.nb;
+  }
+  __device__ __forceinline__ void ask(const Pages& pages, const Pieces& pieces, int kb) {
+    ask(pages, pieces, kb, p0, s0);
+    ask(pages, pieces, kb + BLOCK, p1, s1);
+    ask(pages, pieces, kb + 2 * BLOCK, p2, s2);
+    ask(pages, pieces, kb + 3 * BLOCK, p3, s3);
+  }
+  static __device__ __forceinline__ unsigned of(const Pages& p, int kvh, unsigned page, unsigned sub) {
+    return ((page < (unsigned)p.num_pages ? page : 0u) * p.KV + kvh) * p.nb + sub;
+  }
+};
+
+// The operands of a step as they lie in memory.
+template <int D> struct Held {
+  u32x4_t k[4][D / 64];  // of score tile tt: this lane's key, 16 bytes of every 64 coordinates
+  u32x4_t v[D / 16];     // the lane group's 16 keys of coordinate 16 d + col
+  float ks, vs;
+};
+
+template <int D> __device__ __forceinline__ void load_step(Held<D>& held, const Pages& pages, Blocks b, int kvh) {
+  const int lane = threadIdx.x & (WAVE - 1), col = lane & 15, grp = lane >> 4;
+  const unsigned b0 = Blocks::of(pages, kvh, b.p0, b.s0), b1 = Blocks::of(pages, kvh, b.p1, b.s1);
+  const unsigned b2 = Blocks::of(pages, kvh, b.p2, b.s2), b3 = Blocks::of(pages, kvh, b.p3, b.s3);
+  const unsigned kblock = col & 8 ? (col & 4 ? b3 : b2) : (col & 4 ? b1 : b0), vblock = grp & 2 ? (grp & 1 ? b3 : b2) : (grp & 1 ? b1 : b0);
+  const uint8_t* krow = pages.k + (size_t)kblock * (BLOCK * D) + (col & 3) * D + 16 * grp;
+#pragma unroll
+  for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) held.k[tt][c] = *reinterpret_cast<const u32x4_t*>(krow + 4 * tt * D + 64 * c);
+  held.ks = pages.ks[vblock];
+  held.vs = pages.vs[vblock];
+  const uint8_t* vcol = pages.v + (size_t)vblock * (BLOCK * D) + BLOCK * col;
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d) held.v[d] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(vcol + 16 * BLOCK * d));
+}
+
+// 16 e4m3 values (keys 0 .. 15 of a coordinate) times 2^n as bf16: exact
+__device__ __forceinline__ void widen(const u32x4_t& v, float scale, bf16x8_t (&out)[2]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * h + w], scale, false);
+      const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * h + w], scale, true);
+      out[h][4 * w] = a[0]; out[h][4 * w + 1] = a[1]; out[h][4 * w + 2] = b[0]; out[h][4 * w + 3] = b[1];
+    }
+}
+
+__device__ __forceinline__ float max_of_16(const f32x4_t (&s)[4]) {
+  const float m0 = max3(s[0][0], s[0][1], s[0][2]), m1 = max3(s[0][3], s[1][0], s[1][1]), m2 = max3(s[1][2], s[1][3], s[2][0]);
+  const float m3 = max3(s[2][1], s[2][2], s[2][3]), m4 = max3(s[3][0], s[3][1], s[3][2]);
+  return max3(max3(m0, m1, m2), max3(m3, m4, s[3][3]), NEG_INF);
+}
+
+// A step's products and softmax for queries of one token (pos, lo uniform).  factor: from a score of e4m3 numbers to one in base 2 (natural units where
+// scores are capped), without the block's scale.
+template <int D>
+__device__ __forceinline__ void take_step(const Held<D>& held, int kb, const Query<D>& q, float factor, float cap, int pos, int lo, int keep,
+                                          Running<D>& run) {
+  const int grp = (threadIdx.x & (WAVE - 1)) >> 4;
+  f32x4_t s[4];
+#pragma unroll
+  for (int tt = 0; tt < 4; ++tt) s[tt] = score_tile<D>(held.k[tt], q);
+  float by = factor * fmaxf(held.ks, 0x1p-100f);  // a block that was never written has none; -inf times it stays -inf
+  if (cap > 0.f) {  // uniform
+    by *= __builtin_amdgcn_rcpf(cap);
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[tt][r] = quick_tanh(s[tt][r] * by);
+    by = cap * LOG2E;
+  }
+  if (kb + STEP - 1 > pos || kb < lo) {  // uniform
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int key = kb + 16 * grp + 4 * tt + r;
+        s[tt][r] = key <= pos && (key >= lo || key < keep) ? s[tt][r] : NEG_INF;
+      }
+  }
+  const float mn = fmaxf(run.m, quad_rows_max(max_of_16(s) * by)), base = mn == NEG_INF ? 0.f : mn;
+  const float alpha = __builtin_amdgcn_exp2f(run.m - base);
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  bf16x8_t p[2];
+#pragma unroll
+  for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float w = __builtin_amdgcn_exp2f(fmaf(s[tt][r], by, -base));
+      sum[r] += w;
+      p[tt >> 1][(tt & 1) * 4 + r] = (bf16)w;
+    }
+  run.m = mn;
+  run.l = run.l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+  if (__any(alpha != 1.f)) {
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) run.o[d] *= alpha;
+  }
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d) {
+    bf16x8_t v[2];
+    widen(held.v[d], held.vs, v);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) run.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[h], p[h], run.o[d], 0, 0, 0);
+  }
+}
+
 // A request's pages as its block table names them; entries that are none of the pool's (of pages given back) are read as page 0, and keys beyond
 // `last` as those of its block: numbers, which masks hide.
 struct Table {
@@ -411,6 +533,8 @@ struct Attend {
   float scale;
   Sight sight;
   int part_steps, P;
+  unsigned magic;  // of a page's blocks (`Pieces`)
+  int cus;
 };
 
 __device__ __forceinline__ float score_factor(const Attend& a) { return a.sight.cap > 0.f ? a.scale : a.scale * LOG2E; }
@@ -426,24 +550,56 @@ __device__ __forceinline__ float share_of(const Sight& sight, int head, float m,
 
 // One workgroup per (token, group of query heads, partition of its keys); its four waves take the steps in turn.
 template <int D>
-__global__ __launch_bounds__(256) void single8_kernel(Attend a) {
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a) {
   constexpr int LD = D + 4;
   extern __shared__ __align__(16) float smem[];  // [4][16] m, [4][16] l, [4][G][LD]
-  const int G = a.H / a.KV, item = blockIdx.x, kvh = blockIdx.y, part = blockIdx.z, h0 = kvh * G;
+  const int G = a.H / a.KV, part = blockIdx.z;
+  int item = blockIdx.y, kvh = blockIdx.x;
+  if (a.P == 1) {
+    // Whole contexts of unequal length, a workgroup each, two of them on a compute unit.  Taken eight items at a time, their kv heads one after the
+    // other, with the second round of workgroups backwards: with `items` sorted longest first a compute unit's first two are a long and a short one.
+    int s = blockIdx.x + gridDim.x * blockIdx.y;
+    const int N = gridDim.y, total = N * a.KV;
+    if (s >= a.cus && s < 2 * a.cus) s = a.cus + (min(2 * a.cus, total) - 1 - s);
+    const int first = s / (8 * a.KV) * 8, r = s % (8 * a.KV), here = min(8, N - first);
+    item = first + r % here;
+    kvh = r / here;
+  }
+  const int h0 = kvh * G;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, grp = lane >> 4;
   const int t = a.items ? a.items[item] : item, bs = a.pages.nb * BLOCK;
   const int pos = min(a.positions[t], a.table_width * bs - 1);
   const int lo = first_in_window(a.sight, pos + 1);
-  const Table table{a.tables + (size_t)(a.tok_row ? a.tok_row[t] : t) * a.table_width, pos};
+  const Pieces pieces{a.tables + (size_t)(a.tok_row ? a.tok_row[t] : t) * a.table_width, max(pos, 0) / BLOCK, a.magic};
   const Steps steps(lo, a.sight.keep, pos);
   const int from = part * a.part_steps, to = min(steps.count, from + a.part_steps);
+  // a step's operands are asked for a step ahead, where they lie two steps ahead
+  Held<D> even, odd;
+  Blocks blocks;
+  const int page_head = kvh / a.share;
+  int at = from + wave;
+  if (at < to) {
+    blocks.ask(a.pages, pieces, steps.first_key(at));
+    load_step<D>(even, a.pages, blocks, page_head);
+    if (at + 4 < to) blocks.ask(a.pages, pieces, steps.first_key(at + 4));
+  }
   Running<D> run;
   run.clear();
   Query<D> q;
   load_query<D>(q, a.q + ((size_t)t * a.H + h0 + min(col, G - 1)) * D, grp);
   const float factor = score_factor(a) * q.scale;
-  for (int at = from + wave; at < to; at += 4)
-    step8<D>(a.pages, table, kvh / a.share, steps.first_key(at), q, factor, a.sight.cap, pos, lo, a.sight.keep, run);
+  auto turn = [&](const Held<D>& now, Held<D>& next) {
+    if (at + 4 < to) {
+      load_step<D>(next, a.pages, blocks, page_head);
+      if (at + 8 < to) blocks.ask(a.pages, pieces, steps.first_key(at + 8));
+    }
+    take_step<D>(now, steps.first_key(at), q, factor, a.sight.cap, pos, lo, a.sight.keep, run);
+    at += 4;
+  };
+  while (at < to) {
+    turn(even, odd);
+    if (at < to) turn(odd, even);
+  }
   run.l = quad_rows_sum(run.l);
   float *sm = smem, *sl = smem + 64, *so = smem + 128;
   if (grp == 0 && col < G) { sm[wave * 16 + col] = run.m; sl[wave * 16 + col] = run.l; }
@@ -472,21 +628,32 @@ __global__ __launch_bounds__(256) void single8_kernel(Attend a) {
   }
 }
 
-// The partitions of every (token, head): sum acc_p 2^(m_p - m) / sum l_p 2^(m_p - m).
+// The partitions of every (token, head): sum acc_p 2^(m_p - m) / sum l_p 2^(m_p - m).  A lane holds a partition's weight and hands it round by lane
+// reads: one round of loads for the weights and one, which waits for no other, for the sums.  A thread has a coordinate (D is whole waves).
 __global__ __launch_bounds__(256) void single8_merge_kernel(Attend a, int D) {
-  const int item = blockIdx.x, h = blockIdx.y, t = a.items ? a.items[item] : item;
+  const int item = blockIdx.x, h = blockIdx.y, t = a.items ? a.items[item] : item, lane = threadIdx.x & (WAVE - 1), d = threadIdx.x;
   const size_t base = ((size_t)item * a.H + h) * a.P;
   float m = NEG_INF;
-  for (int p = 0; p < a.P; ++p) m = fmaxf(m, a.part_m[base + p]);
-  for (int d = threadIdx.x; d < D; d += blockDim.x) {
-    float num = 0.f, den = 0.f;
-    for (int p = 0; p < a.P; ++p) {
-      const float e = m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(a.part_m[base + p] - m);
-      num += a.part_acc[(base + p) * D + d] * e;
-      den += a.part_l[base + p] * e;
+  for (int p = lane; p < a.P; p += WAVE) m = fmaxf(m, a.part_m[base + p]);
+  m = wave_max(m);
+  const float* acc = a.part_acc + base * D + d;
+  float num = 0.f, den = 0.f;
+  for (int p0 = 0; p0 < a.P; p0 += WAVE) {
+    const int here = min(WAVE, a.P - p0);
+    const float mp = lane < here ? a.part_m[base + p0 + lane] : NEG_INF;
+    const float weight = mp == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(mp - m), l = weight == 0.f ? 0.f : a.part_l[base + p0 + lane] * weight;
+    for (int p = 0; p < here; p += 8) {  // eight at a time; those past the end repeat the last with a weight of 0
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = acc[(size_t)(p0 + min(p + j, here - 1)) * D];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        den += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(l), p + j));
+        num = fmaf(v[j], __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), p + j)), num);
+      }
     }
-    put(a.out, ((size_t)t * a.H + h) * D + d, num * share_of(a.sight, h, m, den), a.sight.wide);
   }
+  put(a.out, ((size_t)t * a.H + h) * D + d, num * share_of(a.sight, h, m, den), a.sight.wide);
 }
 
 // Portions of prompts: one workgroup per (tile of up to 64 queries, query head), a wave 16 of its queries.
@@ -520,6 +687,12 @@ __global__ __launch_bounds__(256) void prompt8_kernel(Attend a) {
 bool pages_ok(const void* k, const void* v, const float* ks, const float* vs, int num_pages, int KV, int D, int bs) {
   return k && v && ks && vs && num_pages > 0 && KV > 0 && D > 0 && D % 64 == 0 && D <= 256 && bs > 0 && bs % BLOCK == 0 &&
          !(((uintptr_t)k | (uintptr_t)v) & 15);
+}
+// ceil(2^32 / blocks of a page); a page of one block needs none
+unsigned magic_of(int bs) { return bs > BLOCK ? (unsigned)((0x100000000ull + bs / BLOCK - 1) / (bs / BLOCK)) : 0u; }
+bool table_ok(int num_pages, int KV, int bs, int table_width) {  // block numbers fit 32 bits, and their division by a page's is exact
+  const long long nb = bs / BLOCK;
+  return table_width > 0 && (long long)num_pages * KV * nb <= 0xffffffffll && table_width * nb <= 0x7ffffffll && table_width * nb * nb <= 0xffffffffll;
 }
 Pages pages_of(const void* k, const void* v, const float* ks, const float* vs, int num_pages, int KV, int bs) {
   return Pages{(uint8_t*)k, (uint8_t*)v, (float*)ks, (float*)vs, num_pages, KV, bs / BLOCK};
@@ -571,23 +744,23 @@ extern "C" int as_attn_single_query8(const void* q, const void* k_pages, const v
   if (num_items <= 0) return AS_OK;
   const Sight sight{window, keep, chunk, cap, sink, sinks, wide};
   if (!sight_ok(sight) || H <= 0 || KV <= 0 || H % KV || H / KV > 16 || share < 1 || KV % share) return AS_BAD_SHAPE;
-  if (!pages_ok(k_pages, v_pages, k_scales, v_scales, num_pages, KV / share, D, bs) || table_width <= 0) return AS_BAD_SHAPE;
-  if (!q || !positions || !block_tables || !out || part_size <= 0 || part_size % STEP || P <= 0 || P > 65535) return AS_BAD_SHAPE;
+  if (!pages_ok(k_pages, v_pages, k_scales, v_scales, num_pages, KV / share, D, bs) || !table_ok(num_pages, KV / share, bs, table_width)) return AS_BAD_SHAPE;
+  if (!q || !positions || !block_tables || !out || part_size <= 0 || part_size % STEP || P <= 0 || P > 65535 || num_items > 65535) return AS_BAD_SHAPE;
   if (P > 1 && (!part_m || !part_l || !part_acc)) return AS_BAD_SHAPE;
   const Attend a{(const bf16*)q, pages_of(k_pages, v_pages, k_scales, v_scales, num_pages, KV / share, bs), items, positions, tok_row, nullptr,
-                 block_tables, table_width, (bf16*)out, part_m, part_l, part_acc, H, KV, share, scale, sight, part_size / STEP, P};
+                 block_tables, table_width, (bf16*)out, part_m, part_l, part_acc, H, KV, share, scale, sight, part_size / STEP, P, magic_of(bs), compute_units()};
   const size_t shmem = sizeof(float) * (128 + 4 * (size_t)(D + 4) * (H / KV));
 #define LAUNCH(DV)                                                                                                                       \
   {                                                                                                                                      \
     const auto kernel = single8_kernel<DV>;                                                                                              \
     if (shmem > 65536 && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)shmem) != hipSuccess) \
       return AS_LAUNCH_FAILED;                                                                                                           \
-    kernel<<<dim3(num_items, KV, P), 256, shmem, stream>>>(a);                                                                           \
+    kernel<<<dim3(KV, num_items, P), 256, shmem, stream>>>(a);                                                                           \
   }
   FOR_WIDTH(LAUNCH)
 #undef LAUNCH
   if (hipGetLastError() != hipSuccess) return AS_LAUNCH_FAILED;
-  if (P > 1) single8_merge_kernel<<<dim3(num_items, H), D <= 64 ? 64 : D <= 128 ? 128 : 256, 0, stream>>>(a, D);
+  if (P > 1) single8_merge_kernel<<<dim3(num_items, H), D, 0, stream>>>(a, D);
   return launch_status();
 }
 
@@ -599,10 +772,10 @@ extern "C" int as_attn_prefill8(const void* q, const void* k_pages, const void* 
   if (num_tiles <= 0) return AS_OK;
   const Sight sight{window, keep, chunk, cap, sink, sinks, wide};
   if (!sight_ok(sight) || H <= 0 || KV <= 0 || H % KV || H > 65535) return AS_BAD_SHAPE;
-  if (!pages_ok(k_pages, v_pages, k_scales, v_scales, num_pages, KV, D, bs) || table_width <= 0) return AS_BAD_SHAPE;
+  if (!pages_ok(k_pages, v_pages, k_scales, v_scales, num_pages, KV, D, bs) || !table_ok(num_pages, KV, bs, table_width)) return AS_BAD_SHAPE;
   if (!q || !tiles || !block_tables || !out) return AS_BAD_SHAPE;
   const Attend a{(const bf16*)q, pages_of(k_pages, v_pages, k_scales, v_scales, num_pages, KV, bs), nullptr, nullptr, nullptr, tiles, block_tables,
-                 table_width, (bf16*)out, nullptr, nullptr, nullptr, H, KV, 1, scale, sight, 0, 1};
+                 table_width, (bf16*)out, nullptr, nullptr, nullptr, H, KV, 1, scale, sight, 0, 1, magic_of(bs), 0};
 #define LAUNCH(DV) prompt8_kernel<DV><<<dim3(num_tiles, H), 256, 0, stream>>>(a)
   FOR_WIDTH(LAUNCH)
 #undef LAUNCH

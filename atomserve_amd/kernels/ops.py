@@ -903,6 +903,8 @@ def attn_single_query8(q, k_pages, v_pages, k_scales, v_scales, items, positions
         return
     if H % KV or width != D:
         raise KernelError(f"attention over 8 bits: heads {H}/{KV} of {D} do not fit pages of heads of {width}")
+    if not scale > 0:
+        raise KernelError("attention over 8 bits: scores have a positive scale")
     if max_context > block_tables.shape[1] * bs:
         raise KernelError("attention: block tables are shorter than the longest context")
     share = _share8(H // KV)
@@ -925,6 +927,8 @@ def attn_prefill8(q, k_pages, v_pages, k_scales, v_scales, tiles, block_tables, 
         return
     if H % KV or width != D:
         raise KernelError(f"prefill attention over 8 bits: heads {H}/{KV} of {D} do not fit pages of heads of {width}")
+    if not scale > 0:
+        raise KernelError("attention over 8 bits: scores have a positive scale")
     if max_context > block_tables.shape[1] * bs:
         raise KernelError("attention: block tables are shorter than the longest context")
     call("as_attn_prefill8", _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales), NB, _ptr(tiles), tiles.shape[0],
