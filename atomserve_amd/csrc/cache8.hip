@@ -12,6 +12,7 @@
 // rewritten: times a power of two an e4m3 number stays the same number unless it falls under the smallest normal one (2^-15 of the
 // largest), so a block holds what a single rounding gives, however its tokens came.  Integers, or any scale, would be rounded anew each time.
 #include "attn_parts.h"
+#include "wide_tile.h"
 
 namespace {
 
@@ -434,77 +435,6 @@ __device__ __forceinline__ void take_step(const Held<D>& held, int kb, const Que
   }
 }
 
-// A request's pages as its block table names them; entries that are none of the pool's (of pages given back) are read as page 0, and keys beyond
-// `last` as those of its block: numbers, which masks hide.
-struct Table {
-  const int* entries;
-  int last;  // the last key that any column sees
-  __device__ __forceinline__ size_t block_of(const Pages& p, int key, int kvh) const {
-    const int n = min(key, last) / BLOCK, page = entries[n / p.nb];
-    return block_index(p, (unsigned)page < (unsigned)p.num_pages ? page : 0, kvh, n % p.nb);
-  }
-};
-
-// One step: the keys from kb on.  factor: from a score of e4m3 numbers to one in base 2 (natural units where scores are capped), without the block's scale.
-template <int D>
-__device__ __forceinline__ void step8(const Pages& pages, const Table& table, int kvh, int kb, const Query<D>& q, float factor, float cap, int pos,
-                                      int lo, int keep, Running<D>& run) {
-  const int lane = threadIdx.x & (WAVE - 1), col = lane & 15, grp = lane >> 4;
-  const size_t kblock = table.block_of(pages, kb + BLOCK * (col >> 2), kvh), vblock = table.block_of(pages, kb + BLOCK * grp, kvh);
-  f32x4_t s[4];
-  const uint8_t* krow = pages.k + kblock * (BLOCK * D) + (col & 3) * D + 16 * grp;
-#pragma unroll
-  for (int tt = 0; tt < 4; ++tt) {
-    u32x4_t k[D / 64];
-#pragma unroll
-    for (int c = 0; c < D / 64; ++c) k[c] = *reinterpret_cast<const u32x4_t*>(krow + 4 * tt * D + 64 * c);
-    s[tt] = score_tile<D>(k, q);
-  }
-  const float by = factor * pages.ks[vblock], vscale = pages.vs[vblock];
-  float mx = NEG_INF;
-#pragma unroll
-  for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      float v = s[tt][r] * by;
-      if (cap > 0.f) v = cap * LOG2E * quick_tanh(v / cap);
-      const int key = kb + 16 * grp + 4 * tt + r;
-      s[tt][r] = key <= pos && (key >= lo || key < keep) ? v : NEG_INF;
-      mx = fmaxf(mx, s[tt][r]);
-    }
-  const float mn = fmaxf(run.m, quad_rows_max(mx)), base = mn == NEG_INF ? 0.f : mn;
-  const float alpha = __builtin_amdgcn_exp2f(run.m - base);
-  float sum = 0.f;
-  bf16x8_t p[2];
-#pragma unroll
-  for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float w = __builtin_amdgcn_exp2f(s[tt][r] - base);
-      sum += w;
-      p[tt >> 1][(tt & 1) * 4 + r] = (bf16)w;
-    }
-  run.m = mn;
-  run.l = run.l * alpha + sum;
-  const uint8_t* vcol = pages.v + vblock * (BLOCK * D) + BLOCK * col;
-#pragma unroll
-  for (int d = 0; d < D / 16; ++d) {
-    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(vcol + 16 * BLOCK * d);
-    run.o[d] *= alpha;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      bf16x8_t vv;
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * h + w], vscale, false);
-        const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * h + w], vscale, true);
-        vv[4 * w] = a[0]; vv[4 * w + 1] = a[1]; vv[4 * w + 2] = b[0]; vv[4 * w + 3] = b[1];
-      }
-      run.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, p[h], run.o[d], 0, 0, 0);
-    }
-  }
-}
-
 // Which steps of 64 keys a walk takes: those from the sequence's start that hold kept tokens, then those from the first key in sight on.
 struct Steps {
   int kept, base, count;
@@ -517,6 +447,12 @@ struct Steps {
   }
   __device__ __forceinline__ int first_key(int at) const { return STEP * (at < kept ? at : at - kept + base); }
 };
+
+// Four neighbouring results, as bf16 or, with `wide`, fp32.
+__device__ __forceinline__ void put4(bf16* out, size_t i, f32x4_t v, int wide) {
+  if (wide) *reinterpret_cast<f32x4_t*>(reinterpret_cast<float*>(out) + i) = v;
+  else *reinterpret_cast<bf16x4_t*>(out + i) = bf16x4_t{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
+}
 
 struct Attend {
   const bf16* q;
@@ -656,32 +592,317 @@ __global__ __launch_bounds__(256) void single8_merge_kernel(Attend a, int D) {
   put(a.out, ((size_t)t * a.H + h) * D + d, num * share_of(a.sight, h, m, den), a.sight.wide);
 }
 
-// Portions of prompts: one workgroup per (tile of up to 64 queries, query head), a wave 16 of its queries.
-template <int D>
-__global__ __launch_bounds__(256) void prompt8_kernel(Attend a) {
-  const int tile = blockIdx.x, head = blockIdx.y, kvh = head / (a.H / a.KV);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, grp = lane >> 4;
-  const int tok0 = a.tiles[4 * tile], count = a.tiles[4 * tile + 1], pos0 = a.tiles[4 * tile + 3], bs = a.pages.nb * BLOCK;
-  const int q0 = 16 * wave, n = min(16, count - q0);
-  if (n <= 0) return;
-  const int mine = min(col, n - 1), t = tok0 + q0 + mine, end = a.table_width * bs - 1;
-  const int pos = min(pos0 + q0 + mine, end), last = min(pos0 + q0 + n - 1, end);
-  const int lo = first_in_window(a.sight, pos + 1), first = first_in_window(a.sight, pos0 + q0 + 1);
-  const Table table{a.tables + (size_t)a.tiles[4 * tile + 2] * a.table_width, last};
-  const Steps steps(first, a.sight.keep, last);
-  Running<D> run;
-  run.clear();
-  Query<D> q;
-  load_query<D>(q, a.q + ((size_t)t * a.H + head) * D, grp);
-  const float factor = score_factor(a) * q.scale;
-  for (int at = 0; at < steps.count; ++at)
-    step8<D>(a.pages, table, kvh, steps.first_key(at), q, factor, a.sight.cap, pos, lo, a.sight.keep, run);
-  const float inv = share_of(a.sight, head, run.m, quad_rows_sum(run.l));
-  if (col >= n) return;
+// ---- portions of prompts ------------------------------------------------------------------------------------
+//
+// Work item: up to 64 consecutive tokens of one request for one kv head and four waves of queries.  A wave owns 16 QT queries of one head as QT column
+// tiles; the waves of a workgroup take heads of one group or other queries of the tile, so that all need the same keys and values.  Those come into LDS
+// a round of 64 keys ahead, a wave one block of four:
+//
+//   keys     as they are, by copies that pass no register (buffer_load ... lds).  16-byte piece c of key k lies at c ^ swizzle(k): the 16 rows of a
+//            score tile, keys 4 tt .. + 3 of four blocks, lie in different banks.
+//   values   through registers, widened to bf16 on the way (once a workgroup instead of once a wave: the vector unit has the softmax to do):
+//            slot (2 block + h) D + d holds keys 8 h .. + 7 of coordinate d, so that 16 lanes read 256 bytes in one piece.
+//
+// One barrier a round.  Where the blocks lie and their scales are looked up for 16 rounds at a time, a block a lane.
+//
+// A step of few work items takes as long as its longest one: with `pieces` > 1 an item comes as that many workgroups, an item of more than `piece_rounds`
+// rounds is cut along its keys, and what the pieces leave (maxima, sums, unnormalised outputs) is put together by a second kernel.
+struct Cut {
+  int pieces, piece_rounds;
+  int* cut;    // [items]: the pieces of each (1: not cut)
+  float* ml;   // [T, H, pieces, 2] maximum (base 2), sum
+  float* acc;  // [T, H, pieces, D]
+};
+
+template <int D> __device__ __forceinline__ int swizzle(int key) {  // of a key within a round
+  const int block = key >> 4 & 3;
+  return D == 256 ? (key & 3) | block << 2 : D == 128 ? (key >> 1 & 1) | block << 1 : block;
+}
+
+struct Item {  // what a workgroup and a wave of it work on
+  int item, tile, kvh, bz, piece;
+  __device__ __forceinline__ Item(const Attend& a, int units_z, int pass, int pieces) {
+    // Items in the order of `tiles`, those that see most keys first; runs of `pass` of them alternate direction, so that a compute unit that
+    // received one of the longest in one round of workgroups receives one of the shortest in the next.
+    int n = blockIdx.x;
+    const int block = n / pass, first = block * pass, size = min(pass, (int)gridDim.x - first), per_tile = a.KV * units_z;
+    if (block & 1) n = first + size - 1 - (n - first);
+    piece = n % pieces;
+    item = n / pieces;
+    tile = item / per_tile;
+    kvh = item % per_tile / units_z;
+    bz = item % units_z;
+  }
+};
+
+template <int D, int QT>
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt8_kernel(Attend a, int units_z, int pass, Cut cut) {
+  constexpr int DT = D / 16, WQ = 16 * QT, PARTS = 64 / WQ;  // queries of a wave; waves that share a head's 64 queries
+  constexpr int KEYS = STEP * D, VALUES = 2 * STEP * D;      // bytes of a round
+  __shared__ __align__(128) char keys[2][KEYS];
+  __shared__ __align__(128) char values[2][VALUES];
+  const Item it(a, units_z, pass, cut.pieces);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, grp = lane >> 4;
+  const int G = a.H / a.KV, kvh = it.kvh, end = a.table_width * a.pages.nb * BLOCK - 1;
+  const int tok0 = a.tiles[4 * it.tile], count = a.tiles[4 * it.tile + 1], pos0 = max(a.tiles[4 * it.tile + 3], 0);
+  const int* const table = a.tables + (size_t)a.tiles[4 * it.tile + 2] * a.table_width;
+  auto first_seen = [&](int pos) { return first_in_window(a.sight, pos + 1); };
+
+  // the keys this workgroup walks: from the first key that any of its waves sees to the last
+  int wg_lo = 0x7fffffff, wg_last = -1;
+  for (int u = it.bz * 4; u < it.bz * 4 + 4 && u < PARTS * G; ++u) {
+    const int uq0 = u / G * WQ;
+    if (uq0 >= count) continue;
+    wg_last = max(wg_last, min(pos0 + min(count, uq0 + WQ) - 1, end));
+    wg_lo = min(wg_lo, first_seen(min(pos0 + uq0, end)));
+  }
+  if (wg_last < 0) {  // uniform over the workgroup
+    if (cut.pieces > 1 && it.piece == 0 && tid == 0) cut.cut[it.item] = 1;
+    return;
+  }
+  const int keep = a.sight.keep;
+  const Steps steps(wg_lo, keep, wg_last);
+  int rd_first = 0, rd_end = steps.count;
+  bool partial = false;  // this workgroup leaves its share of a cut item for the merge
+  if (cut.pieces > 1) {
+    const int mine = min(cut.pieces, (rd_end + cut.piece_rounds - 1) / cut.piece_rounds);
+    if (it.piece == 0 && tid == 0) cut.cut[it.item] = mine;
+    if (it.piece >= mine) return;
+    if (mine > 1) {
+      partial = true;
+      rd_first = cut.piece_rounds * it.piece;
+      if (it.piece + 1 < mine) rd_end = rd_first + cut.piece_rounds;
+    }
+  }
+  const int rounds = rd_end - rd_first;
+
+  // this wave's queries
+  const int unit = it.bz * 4 + wave, head = kvh * G + unit % G, q0 = unit / G * WQ;
+  const bool working = unit < PARTS * G && q0 < count;
+  const int nq = working ? min(WQ, count - q0) : 1;
+  const int my_first = min(pos0 + q0, end), my_last = working ? min(pos0 + q0 + nq - 1, end) : -1;
+  const int my_lo = first_seen(my_first), last_lo = first_seen(my_last);
+  Query<D> q[QT];
+  Running<D> run[QT];
+  int qpos[QT], qlo[QT];
+  float factor[QT];
 #pragma unroll
-  for (int d = 0; d < D / 16; ++d)
+  for (int qt = 0; qt < QT; ++qt) {
+    const int qc = min(qt * 16 + col, nq - 1);  // columns past the end repeat the last query and are not stored
+    qpos[qt] = min(pos0 + q0 + qc, end);
+    qlo[qt] = first_seen(qpos[qt]);
+    load_query<D>(q[qt], a.q + ((size_t)(tok0 + (working ? q0 + qc : 0)) * a.H + head) * D, grp);
+    factor[qt] = score_factor(a) * q[qt].scale;
+    run[qt].clear();
+  }
+
+  // where blocks lie: lane l has block l % 4 of round 16 batch + l / 4
+  const int last_block = wg_last / BLOCK;
+  auto place_of = [&](int batch) {
+    const int rd = min(16 * batch + (lane >> 2), rounds - 1);
+    return min(steps.first_key(rd_first + rd) / BLOCK + (lane & 3), last_block);
+  };
+  auto entry_of = [&](int n) { return a.pages.nb == 1 ? n : (int)__umulhi(n, a.magic); };
+  int page_ahead = table[entry_of(place_of(0))];
+  unsigned block = 0;
+  float ks_ahead = 0.f, vs_ahead = 0.f;
+  auto locate = [&](int batch) {
+    const int n = place_of(batch);
+    const unsigned page = (unsigned)page_ahead < (unsigned)a.pages.num_pages ? page_ahead : 0u;
+    block = (page * a.pages.KV + kvh) * a.pages.nb + (n - entry_of(n) * a.pages.nb);
+    ks_ahead = a.pages.ks[block];
+    vs_ahead = a.pages.vs[block];
+    page_ahead = table[entry_of(place_of(batch + 1))];
+  };
+
+  // this wave's share of a round: block `wave` of four
+  int k_at[D / 64];  // the byte of a block that this lane copies
 #pragma unroll
-    for (int r = 0; r < 4; ++r) put(a.out, ((size_t)t * a.H + head) * D + 16 * d + 4 * grp + r, run.o[d][r] * inv, a.sight.wide);
+  for (int i = 0; i < D / 64; ++i) {
+    const int slot = 64 * i + lane, key = slot / (D / 16), c = slot % (D / 16);
+    k_at[i] = key * D + (c ^ swizzle<D>(16 * wave + key)) * 16;
+  }
+  u32x4_t raw[D / 64];  // values on their way
+  size_t at = 0;
+  auto aim = [&](int rd) {
+    if ((rd & 15) == 0) locate(rd >> 4);
+    at = (size_t)(unsigned)__builtin_amdgcn_readlane(block, 4 * (rd & 15) + wave) * (BLOCK * D);
+  };
+  auto copy_keys = [&](int rd) {
+    const __amdgpu_buffer_rsrc_t buf = __builtin_amdgcn_make_buffer_rsrc(a.pages.k + at, 0, BLOCK * D, 0x00020000);
+    const unsigned to = (unsigned)(uintptr_t)(wide::lds_char*)&keys[rd & 1][wave * BLOCK * D];
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) wide::copy_to_lds(buf, k_at[i], 0u, to + 1024 * i);
+  };
+  auto ask_values = [&]() {
+    const u32x4_t* from = reinterpret_cast<const u32x4_t*>(a.pages.v + at) + lane;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) raw[i] = from[64 * i];
+  };
+  auto put_values = [&](int rd) {  // the block's scale is the wave's own: lane 4 r + wave of the batch
+    const float scale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs_ahead), 4 * (rd & 15) + wave));
+    u32x4_t* const to = reinterpret_cast<u32x4_t*>(values[rd & 1]) + 2 * wave * D + lane;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      bf16x8_t v[2];
+      widen(raw[i], scale, v);
+      to[64 * i] = __builtin_bit_cast(u32x4_t, v[0]);
+      to[64 * i + D] = __builtin_bit_cast(u32x4_t, v[1]);
+    }
+  };
+  const int swz = swizzle<D>(16 * (col >> 2) + (col & 3));
+  const char* const krow = keys[0] + (16 * (col >> 2) + (col & 3)) * D;
+
+  float ks_now = 0.f;
+  aim(0);
+  copy_keys(0);
+  ask_values();
+  put_values(0);
+  for (int rd = 0; rd < rounds; ++rd) {
+    if ((rd & 15) == 0) ks_now = ks_ahead;  // the batch that this round belongs to, before the copies' next one
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const bool more = rd + 1 < rounds;
+    if (more) {
+      aim(rd + 1);
+      copy_keys(rd + 1);
+      ask_values();
+    }
+    const int kb = steps.first_key(rd_first + rd);
+    if (working && kb <= my_last && (kb + STEP - 1 >= my_lo || kb < keep)) {  // uniform over the wave
+      const float ks = __shfl(ks_now, 4 * (rd & 15) + grp, WAVE);
+      f32x4_t s[QT][4];
+      u32x4_t k[2][D / 64];
+      auto read_keys = [&](int tt, u32x4_t (&into)[D / 64]) {
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) into[c] = *reinterpret_cast<const u32x4_t*>(krow + (rd & 1) * KEYS + 4 * tt * D + ((4 * c + grp) ^ swz) * 16);
+      };
+      read_keys(0, k[0]);
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {
+        if (tt < 3) read_keys(tt + 1, k[(tt + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);  // or the compiler moves every read down to its product
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) s[qt][tt] = score_tile<D>(k[tt & 1], q[qt]);
+      }
+      u32x4_t v[2][DT];
+      auto read_values = [&](int h) {
+        const u32x4_t* from = reinterpret_cast<const u32x4_t*>(values[rd & 1]) + (2 * grp + h) * D + col;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) v[h][d] = from[16 * d];
+      };
+      constexpr bool EARLY = D <= 128;  // asked for before the softmax, as far as registers hold them
+      if constexpr (EARLY) read_values(0);
+      __builtin_amdgcn_sched_barrier(0);
+      const bool masked = kb + STEP - 1 > my_first || kb < last_lo;
+      bf16x8_t p[QT][2];
+      float alpha[QT];
+      bool rescale = false;
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        float by = factor[qt] * fmaxf(ks, 0x1p-100f);
+        if (a.sight.cap > 0.f) {
+          by *= __builtin_amdgcn_rcpf(a.sight.cap);
+#pragma unroll
+          for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[qt][tt][r] = quick_tanh(s[qt][tt][r] * by);
+          by = a.sight.cap * LOG2E;
+        }
+        if (masked) {
+#pragma unroll
+          for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int key = kb + 16 * grp + 4 * tt + r;
+              s[qt][tt][r] = key <= qpos[qt] && (key >= qlo[qt] || key < keep) ? s[qt][tt][r] : NEG_INF;
+            }
+        }
+        const float mn = fmaxf(run[qt].m, quad_rows_max(max_of_16(s[qt]) * by)), base = mn == NEG_INF ? 0.f : mn;
+        alpha[qt] = __builtin_amdgcn_exp2f(run[qt].m - base);
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float w = __builtin_amdgcn_exp2f(fmaf(s[qt][tt][r], by, -base));
+            sum[r] += w;
+            p[qt][tt >> 1][(tt & 1) * 4 + r] = (bf16)w;
+          }
+        run[qt].m = mn;
+        run[qt].l = run[qt].l * alpha[qt] + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        rescale = rescale || alpha[qt] != 1.f;
+      }
+      if (__any(rescale)) {  // some query's maximum moved: rare once the first keys have been seen
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+          for (int d = 0; d < DT; ++d) run[qt].o[d] *= alpha[qt];
+      }
+      if constexpr (!EARLY) read_values(0);
+      read_values(1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt)
+            run[qt].o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, v[h][d]), p[qt][h], run[qt].o[d], 0, 0, 0);
+    }
+    if (more) put_values(rd + 1);
+  }
+
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const float l = quad_rows_sum(run[qt].l);
+    if (!working || qt * 16 + col >= nq) continue;
+    const size_t row = (size_t)(tok0 + q0 + qt * 16 + col) * a.H + head;
+    if (partial) {
+      const size_t to = row * cut.pieces + it.piece;
+      if (grp == 0) *reinterpret_cast<float2*>(cut.ml + 2 * to) = make_float2(run[qt].m, l);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4_t*>(cut.acc + to * D + 16 * d + 4 * grp) = run[qt].o[d];
+      continue;
+    }
+    const float inv = share_of(a.sight, head, run[qt].m, l);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) put4(a.out, row * D + 16 * d + 4 * grp, run[qt].o[d] * inv, a.sight.wide);
+  }
+}
+
+// The pieces of every cut item, put together: out = sum_j acc_j 2^(m_j - m) / sum_j l_j 2^(m_j - m).  One workgroup per item, lanes as above.
+template <int D, int QT>
+__global__ __launch_bounds__(256) void prompt8_merge_kernel(Attend a, int units_z, Cut cut) {
+  constexpr int WQ = 16 * QT, PARTS = 64 / WQ;
+  const int item = blockIdx.x, n = cut.cut[item];
+  if (n <= 1) return;
+  const int G = a.H / a.KV, per_tile = a.KV * units_z, tile = item / per_tile, kvh = item % per_tile / units_z, bz = item % units_z;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
+  const int tok0 = a.tiles[4 * tile], count = a.tiles[4 * tile + 1];
+  const int unit = bz * 4 + wave, head = kvh * G + unit % G, q0 = unit / G * WQ;
+  if (unit >= PARTS * G || q0 >= count) return;
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const int qi = q0 + qt * 16 + col;
+    if (qi >= count) continue;
+    const size_t row = (size_t)(tok0 + qi) * a.H + head, from = row * cut.pieces;
+    const float2* ml = reinterpret_cast<const float2*>(cut.ml) + from;
+    float m = NEG_INF, den = 0.f;
+    for (int j = 0; j < n; ++j) m = fmaxf(m, ml[j].x);
+    f32x4_t sum[D / 16];
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) sum[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < n; ++j) {
+      const float2 part = ml[j];
+      const float w = part.x == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(part.x - m);
+      den += part.y * w;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) sum[d] += *reinterpret_cast<const f32x4_t*>(cut.acc + (from + j) * D + 16 * d + 4 * grp) * w;
+    }
+    const float inv = share_of(a.sight, head, m, den);
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) put4(a.out, row * D + 16 * d + 4 * grp, sum[d] * inv, a.sight.wide);
+  }
 }
 
 bool pages_ok(const void* k, const void* v, const float* ks, const float* vs, int num_pages, int KV, int D, int bs) {
@@ -764,20 +985,36 @@ extern "C" int as_attn_single_query8(const void* q, const void* k_pages, const v
   return launch_status();
 }
 
-// Portions of prompts: tiles [num_tiles, 4] int32 (first token, count <= 64, row of block_tables, position of the first).
+// Portions of prompts: tiles [num_tiles, 4] int32 (first token, count <= 64, row of block_tables, position of the first), best those that see most keys
+// first.  query_tiles: 2, a wave owns 32 queries of a head; 1, 16 (twice the workgroups).  pieces > 1: items of more than piece_rounds rounds of 64 keys
+// are cut; cut [num_tiles * KV * ceil(64 / (16 query_tiles) * (H / KV) / 4)] int32, part_ml [T, H, pieces, 2] and part_acc [T, H, pieces, D] fp32 with T one
+// more than the largest token of a tile; piece_rounds * pieces covers the longest item.  pieces <= 1: none is cut, the three may be null.
 extern "C" int as_attn_prefill8(const void* q, const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
                                 int num_pages, const int* tiles, int num_tiles, const int* block_tables, int table_width, void* out, int H,
                                 int KV, int D, int bs, float scale, int window, int keep, int chunk, float cap, int sink, const float* sinks,
-                                int wide, hipStream_t stream) {
+                                int wide, int query_tiles, int pieces, int piece_rounds, int* cut, float* part_ml, float* part_acc,
+                                hipStream_t stream) {
   if (num_tiles <= 0) return AS_OK;
   const Sight sight{window, keep, chunk, cap, sink, sinks, wide};
-  if (!sight_ok(sight) || H <= 0 || KV <= 0 || H % KV || H > 65535) return AS_BAD_SHAPE;
+  if (!sight_ok(sight) || H <= 0 || KV <= 0 || H % KV || (query_tiles != 1 && query_tiles != 2)) return AS_BAD_SHAPE;
   if (!pages_ok(k_pages, v_pages, k_scales, v_scales, num_pages, KV, D, bs) || !table_ok(num_pages, KV, bs, table_width)) return AS_BAD_SHAPE;
   if (!q || !tiles || !block_tables || !out) return AS_BAD_SHAPE;
+  if (pieces < 1) pieces = 1;
+  if (pieces > 1 && (piece_rounds < 1 || !cut || !part_ml || !part_acc)) return AS_BAD_SHAPE;
+  const int units_z = (64 / (16 * query_tiles) * (H / KV) + 3) / 4;
+  const long long items = (long long)num_tiles * KV * units_z;
+  if (items * pieces > 0x7fffffffll) return AS_BAD_SHAPE;
   const Attend a{(const bf16*)q, pages_of(k_pages, v_pages, k_scales, v_scales, num_pages, KV, bs), nullptr, nullptr, nullptr, tiles, block_tables,
-                 table_width, (bf16*)out, nullptr, nullptr, nullptr, H, KV, 1, scale, sight, 0, 1, magic_of(bs), 0};
-#define LAUNCH(DV) prompt8_kernel<DV><<<dim3(num_tiles, H), 256, 0, stream>>>(a)
+                 table_width, (bf16*)out, nullptr, nullptr, nullptr, H, KV, 1, scale, sight, 0, 1, magic_of(bs), compute_units()};
+  const Cut how{pieces, piece_rounds, cut, part_ml, part_acc};
+#define LAUNCH2(DV, QTV)                                                                                           \
+  {                                                                                                                \
+    prompt8_kernel<DV, QTV><<<(int)(items * pieces), 256, 0, stream>>>(a, units_z, compute_units(), how);          \
+    if (pieces > 1) prompt8_merge_kernel<DV, QTV><<<(int)items, 256, 0, stream>>>(a, units_z, how);                \
+  }
+#define LAUNCH(DV) if (query_tiles == 1) LAUNCH2(DV, 1) else LAUNCH2(DV, 2)
   FOR_WIDTH(LAUNCH)
 #undef LAUNCH
+#undef LAUNCH2
   return launch_status();
 }

@@ -914,8 +914,8 @@ def attn_single_query8(q, k_pages, v_pages, k_scales, v_scales, items, positions
          float(scale), *sight, part_size, P, share, _stream())  # fmt: skip
 
 
-def attn_prefill8(q, k_pages, v_pages, k_scales, v_scales, tiles, block_tables, out, scale, window, max_context, tile_keys: int = 0, keep_first=0,
-                  softcap=0.0, sink=False, chunk=0) -> None:  # fmt: skip
+def attn_prefill8(q, k_pages, v_pages, k_scales, v_scales, tiles, block_tables, out, scale, window, max_context, query_tiles=None,
+                  tile_keys: int = 0, keep_first=0, softcap=0.0, sink=False, chunk=0) -> None:  # fmt: skip
     """`attn_prefill` over a cache in 8 bits: arguments as there."""
     _check(q, "q", BF16, (None, None, None))
     T, H, D = q.shape
@@ -931,8 +931,15 @@ def attn_prefill8(q, k_pages, v_pages, k_scales, v_scales, tiles, block_tables, 
         raise KernelError("attention over 8 bits: scores have a positive scale")
     if max_context > block_tables.shape[1] * bs:
         raise KernelError("attention: block tables are shorter than the longest context")
+    query_tiles, pieces, piece_rounds = _prefill_plan(tiles.shape[0], H, KV, D, max_context, window or chunk, query_tiles, tile_keys, sight[1])
+    cut = part_ml = part_acc = None
+    if pieces > 1:
+        cut = torch.empty(tiles.shape[0] * KV * _prefill_units(query_tiles, H // KV), dtype=I32, device=q.device)
+        part_ml = torch.empty((T, H, pieces, 2), dtype=F32, device=q.device)
+        part_acc = torch.empty((T, H, pieces, D), dtype=F32, device=q.device)
     call("as_attn_prefill8", _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales), NB, _ptr(tiles), tiles.shape[0],
-         _ptr(block_tables), block_tables.shape[1], _ptr(out), H, KV, D, bs, float(scale), *sight, _stream())  # fmt: skip
+         _ptr(block_tables), block_tables.shape[1], _ptr(out), H, KV, D, bs, float(scale), *sight, int(query_tiles), pieces, piece_rounds, _ptr(cut),
+         _ptr(part_ml), _ptr(part_acc), _stream())  # fmt: skip
 
 
 SKINNY_MAX_ROWS = 16  # up to here the bf16 product streams the weights through our own kernel

@@ -315,6 +315,18 @@ def test_prompts_masks(ops, kw):
     prompt(ops, 8, 2, 128, 16, [(70, 130), (9, 3)], **kw)
 
 
+@pytest.mark.parametrize("query_tiles", [1, 2])
+@pytest.mark.parametrize("pieces", [1, 2, 5])
+@pytest.mark.parametrize("kw", [{}, {"window": 300, "keep_first": 70}, {"sink": True, "softcap": 9.0}, {"chunk": 200, "out_dtype": F32}], ids=str)
+def test_prompts_cut_along_their_keys(ops, monkeypatch, query_tiles, pieces, kw):
+    """Items of every length in a step that is cut: the short ones stay whole."""
+    monkeypatch.setattr(ops, "PREFILL_PIECES", pieces)
+    ops._prefill_plan_of.cache_clear()
+    prompt(ops, 6, 2, 64, 32, [(100, 1500), (70, 0), (5, 700), (64, 192)], query_tiles=query_tiles, **kw)
+    prompt(ops, 10, 2, 128, 16, [(65, 1100), (40, 20)], query_tiles=query_tiles, **kw)
+    ops._prefill_plan_of.cache_clear()
+
+
 def test_prompts_longer(ops):
     prompt(ops, 16, 8, 128, 16, [(500, 0), (200, 3000)])
     prompt(ops, 32, 8, 128, 16, [(64, 6000)])
