@@ -55,29 +55,32 @@ __device__ __forceinline__ size_t block_index(const Pages& p, int page, int kvh,
 
 // ---- appending ------------------------------------------------------------------------------------------
 //
-// One wave per (token, some query heads) and per (run of tokens of a block, kv head, keys or values).  A run: tokens next to each other in the
-// step that go to places next to each other of one block; its first token's wave does all of it, the others' leave.  A wave's lanes take a
-// token's head in pieces of four coordinates, 64 / LPT tokens (or query heads) at a time.
+// A head is D / 8 lanes' work: lane j < R / 8 has the pairs 4 j .. 4 j + 3 of its rotation (coordinates i and i + R/2), the others eight coordinates that
+// are not turned; no lane needs another's but for the sum of squares.
+//
+// Queries: a group of lanes a (token, head), heads side by side.  Keys and values: a wave takes the runs that start among `chunk` neighbouring tokens, for
+// one kv head's keys or values.  A run: tokens next to each other in the step that go to places next to each other of one block, so that one wave sees
+// all that the step puts there: the largest magnitude, the scale, and what the block held.  Lane group s has the run's places PASSES s .. + PASSES - 1 of the
+// block, so that a coordinate's bytes are neighbours in a lane's hands: they cross to the transposed block through LDS.
 template <int D> struct Lanes {
-  static constexpr int LPT = D <= 64 ? 16 : D <= 128 ? 32 : 64;  // lanes of a head, D / 4 of them busy
+  static constexpr int LPT = D <= 64 ? 8 : D <= 128 ? 16 : 32;  // lanes of a head, D / 8 of them busy
   static constexpr int AT_ONCE = WAVE / LPT, PASSES = BLOCK / AT_ONCE;
 };
 
 template <int LPT> __device__ __forceinline__ float lanes_sum(float v) {
-  if constexpr (LPT == 64) v = plus_32(v);
   if constexpr (LPT >= 32) v = plus_16(v);
-  v += dpp<DPP_ROTATE(8)>(v);
-  v += dpp<DPP_ROTATE(4)>(v);
+  if constexpr (LPT >= 16) v += dpp<DPP_ROTATE(8)>(v);
+  v += dpp<DPP_XOR_1>(v);
   v += dpp<DPP_XOR_2>(v);
-  return v + dpp<DPP_XOR_1>(v);
+  return v + dpp<DPP_HALF_MIRROR>(v);
 }
 
-__device__ __forceinline__ void load4(const bf16* p, float (&x)[4]) {
+__device__ __forceinline__ void load4(const bf16* p, float* x) {
   const uint2 r = *reinterpret_cast<const uint2*>(p);
   x[0] = __uint_as_float(r.x << 16); x[1] = __uint_as_float(r.x & 0xffff0000u);
   x[2] = __uint_as_float(r.y << 16); x[3] = __uint_as_float(r.y & 0xffff0000u);
 }
-__device__ __forceinline__ void load4(const float* p, float (&x)[4]) {
+__device__ __forceinline__ void load4(const float* p, float* x) {
   const float4 r = *reinterpret_cast<const float4*>(p);
   x[0] = r.x; x[1] = r.y; x[2] = r.z; x[3] = r.w;
 }
@@ -92,122 +95,137 @@ struct Append {
   Pages pages;
   int T, H, R;
   float eps;
+  int chunk, kv_blocks;  // tokens whose runs a wave takes; workgroups of keys and values, which come first
 };
 
-// x: four coordinates of a head per lane; norm (w: gains) and rotation by the angles of token t.
-template <int D, typename W>
-__device__ __forceinline__ void norm_turn(float (&x)[4], const W* w, const float2* cs, float eps, int R, int t, int j) {
-  constexpr int LPT = Lanes<D>::LPT;
-  const bool busy = 4 * j < D;
-  if (w) {
-    const float ss = lanes_sum<LPT>(busy ? x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3] : 0.f);
-    const float inv = 1.0f / sqrtf(ss / (float)D + eps);
-    float g[4] = {0.f, 0.f, 0.f, 0.f};
-    if (busy) load4(w + 4 * j, g);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = x[i] * inv * g[i];
+// The two pieces of four coordinates of lane j of a head whose first R coordinates turn.
+struct Places {
+  int a, b;
+  __device__ __forceinline__ Places(int j, int R) {
+    const bool turns = 8 * j < R;
+    a = turns ? 4 * j : 8 * j;
+    b = turns ? 4 * j + R / 2 : 8 * j + 4;
   }
-  if (cs) {
-    const int half = R / 8;  // in pieces of four
-    const bool first = j < half, turns = j < 2 * half;
-    const int other = (threadIdx.x & (WAVE - 1)) + (first ? half : turns ? -half : 0);
-    float y[4];
+};
+
+// Norm (gains g, or none) and rotation of a head's eight coordinates in this lane by the angles of token t.
+template <int D>
+__device__ __forceinline__ void norm_turn(float (&x)[8], bool norm, const float (&g)[8], const float2* cs, float eps, int R, int t, int j) {
+  if (norm) {
+    float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = __shfl(x[i], other, WAVE);
-    if (turns) {
-      const float4* angles = reinterpret_cast<const float4*>(cs + (size_t)t * (R / 2) + 4 * (first ? j : j - half));
-      const float4 a = angles[0], b = angles[1];
-      const float c[4] = {a.x, a.z, b.x, b.z}, s[4] = {a.y, a.w, b.y, b.w};
+    for (int i = 0; i < 8; ++i) ss += x[i] * x[i];  // 0 in lanes without coordinates
+    const float inv = 1.0f / sqrtf(lanes_sum<Lanes<D>::LPT>(ss) / (float)D + eps);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = first ? x[i] * c[i] - y[i] * s[i] : x[i] * c[i] + y[i] * s[i];
+    for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * g[i];
+  }
+  if (8 * j < R) {
+    const float4* angles = reinterpret_cast<const float4*>(cs + (size_t)t * (R / 2) + 4 * j);
+    const float4 a = angles[0], b = angles[1];
+    const float c[4] = {a.x, a.z, b.x, b.z}, s[4] = {a.y, a.w, b.y, b.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float u = x[i], v = x[4 + i];
+      x[i] = u * c[i] - v * s[i];
+      x[4 + i] = v * c[i] + u * s[i];
     }
   }
 }
 
-template <int D, typename W>
-__global__ __launch_bounds__(WAVE) void append8_kernel(Append a) {
-  constexpr int LPT = Lanes<D>::LPT, AT_ONCE = Lanes<D>::AT_ONCE, PASSES = Lanes<D>::PASSES;
-  __shared__ __align__(16) uint8_t turned[D * BLOCK];  // values of a run, transposed
-  const int t = blockIdx.x, lane = threadIdx.x, sub = lane / LPT, j = lane % LPT;
-  const int q_units = (a.H + AT_ONCE - 1) / AT_ONCE, KV = a.pages.KV, heads = a.H + 2 * KV;
-  const bool busy = 4 * j < D;
-  int unit = blockIdx.y;
-  if (unit < q_units) {
-    const int h = unit * AT_ONCE + sub;
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    if (busy && h < a.H) load4(a.qkv + ((size_t)t * heads + h) * D + 4 * j, x);
-    norm_turn<D, W>(x, (const W*)a.qw, a.cs, a.eps, a.R, t, j);
-    if (busy && h < a.H) {
-      const bf16x4_t r = {(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]};
-      *reinterpret_cast<bf16x4_t*>(a.q_out + ((size_t)t * a.H + h) * D + 4 * j) = r;
-    }
-    return;
+template <int D, typename W> __device__ __forceinline__ void append_query(const Append& a, unsigned unit, int j) {
+  const int t = unit / a.H, h = unit - t * a.H;
+  if (t >= a.T) return;  // whole groups leave
+  const bool busy = 8 * j < D;
+  const Places at(busy ? j : 0, a.R);
+  const bf16* src = a.qkv + ((size_t)t * (a.H + 2 * a.pages.KV) + h) * D;
+  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, g[8];
+  if (busy) {
+    load4(src + at.a, x);
+    load4(src + at.b, x + 4);
   }
-  unit -= q_units;
-  const bool values = unit >= KV;
-  const int kvh = values ? unit - KV : unit;
-  const int slot = a.slots[t], bs = a.pages.nb * BLOCK;
-  if (slot < 0 || slot / bs >= a.pages.num_pages) return;
-  const int off = slot % BLOCK;
-  if (off > 0 && t > 0 && a.slots[t - 1] == slot - 1) return;  // an earlier token's run
-  const int most = min(BLOCK - off, a.T - t);
-  const bool goes_on = lane < most && a.slots[min(t + lane, a.T - 1)] == slot + lane;
-  const int n = __builtin_ctzll(~__ballot(goes_on));  // tokens of the run
-  const size_t block = block_index(a.pages, slot / bs, kvh, slot % bs / BLOCK);
+  if (a.qw) {
+    load4((const W*)a.qw + at.a, g);
+    load4((const W*)a.qw + at.b, g + 4);
+  }
+  norm_turn<D>(x, a.qw != nullptr, g, a.cs, a.eps, busy ? a.R : 0, t, j);
+  if (!busy) return;
+  bf16* dst = a.q_out + ((size_t)t * a.H + h) * D;
+  *reinterpret_cast<bf16x4_t*>(dst + at.a) = bf16x4_t{(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]};
+  *reinterpret_cast<bf16x4_t*>(dst + at.b) = bf16x4_t{(bf16)x[4], (bf16)x[5], (bf16)x[6], (bf16)x[7]};
+}
 
-  float x[PASSES][4], amax = 0.f;
-  const bf16* src = a.qkv + ((size_t)t * heads + a.H + unit) * D + 4 * j;
+// A run of n tokens from token t on into the places from `off` on of a block.  turned: D * 16 bytes of LDS, this wave's own.
+template <int D, typename W, bool VALUES>
+__device__ __forceinline__ void append_run(const Append& a, int t, int n, int slot, int kvh, const float (&g)[8], uint8_t* turned) {
+  constexpr int LPT = Lanes<D>::LPT, PASSES = Lanes<D>::PASSES;
+  const int lane = threadIdx.x & (WAVE - 1), group = lane / LPT, j = lane % LPT, heads = a.H + 2 * a.pages.KV, bs = a.pages.nb * BLOCK;
+  const bool busy = 8 * j < D;
+  const int R = VALUES ? 0 : a.R, off = slot % BLOCK;
+  const Places at(busy ? j : 0, R);
+  const size_t block = block_index(a.pages, slot / bs, kvh, slot % bs / BLOCK);
+  const bf16* src = a.qkv + ((size_t)t * heads + a.H + (VALUES ? a.pages.KV : 0) + kvh) * D;
+  float x[PASSES][8], amax = 0.f;
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
+    const int nth = group * PASSES + p - off;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[p][i] = 0.f;
-    const int nth = p * AT_ONCE + sub;
-    if (busy && nth < n) load4(src + (size_t)nth * heads * D, x[p]);
+    for (int i = 0; i < 8; ++i) x[p][i] = 0.f;
+    if (busy && nth >= 0 && nth < n) {
+      load4(src + (size_t)nth * heads * D + at.a, x[p]);
+      load4(src + (size_t)nth * heads * D + at.b, x[p] + 4);
+    }
   }
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    if (!values && p * AT_ONCE < n)  // uniform
-      norm_turn<D, W>(x[p], (const W*)a.kw, a.cs, a.eps, a.R, t + min(p * AT_ONCE + sub, n - 1), j);
+    const int nth = group * PASSES + p - off;
+    if constexpr (!VALUES) {
+      if (__any(nth >= 0 && nth < n)) norm_turn<D>(x[p], a.kw != nullptr, g, a.cs, a.eps, busy ? R : 0, t + min(max(nth, 0), n - 1), j);
+    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       x[p][i] = finite_or_zero(x[p][i]);
       amax = fmaxf(amax, fabsf(x[p][i]));
     }
   }
   amax = wave_max(amax);
-  float* scales = values ? a.pages.vs : a.pages.ks;
+  float* scales = VALUES ? a.pages.vs : a.pages.ks;
   const float before = off > 0 ? scales[block] : 0.f;  // a block that begins with this run is new
   const float scale = fmaxf(before, block_scale(amax)), inv = inverse_of(scale);
   const bool grows = before > 0.f && scale > before;
   const float by = before * inv;
-  uint8_t* at = (values ? a.pages.v : a.pages.k) + block * (BLOCK * D);
-  if (!values) {
+  uint8_t* base = (VALUES ? a.pages.v : a.pages.k) + block * (BLOCK * D);
+  if constexpr (!VALUES) {
     if (grows) {  // the block's other rows at the new scale
       for (int w = lane; w < BLOCK * D / 4; w += WAVE) {
         const int row = 4 * w / D;
-        unsigned* word = reinterpret_cast<unsigned*>(at) + w;
+        unsigned* word = reinterpret_cast<unsigned*>(base) + w;
         if (row < off || row >= off + n) *word = rescale4(*word, by);
       }
     }
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
-      const int nth = p * AT_ONCE + sub;
-      if (busy && nth < n)
-        *reinterpret_cast<unsigned*>(at + (off + nth) * D + 4 * j) = pack4(x[p][0] * inv, x[p][1] * inv, x[p][2] * inv, x[p][3] * inv);
-    }
-  } else {
-#pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-      const int nth = p * AT_ONCE + sub;
-      if (busy && nth < n) {
-        const unsigned w = pack4(x[p][0] * inv, x[p][1] * inv, x[p][2] * inv, x[p][3] * inv);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) turned[(4 * j + i) * BLOCK + off + nth] = (uint8_t)(w >> (8 * i));
+      const int place = group * PASSES + p;
+      if (busy && place >= off && place < off + n) {
+        *reinterpret_cast<unsigned*>(base + place * D + at.a) = pack4(x[p][0] * inv, x[p][1] * inv, x[p][2] * inv, x[p][3] * inv);
+        *reinterpret_cast<unsigned*>(base + place * D + at.b) = pack4(x[p][4] * inv, x[p][5] * inv, x[p][6] * inv, x[p][7] * inv);
       }
     }
-    __syncthreads();
-    // which bytes of a coordinate's 16 are the run's
-    u32x4_t mine;
+  } else {
+    if (busy) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint8_t* to = turned + (8 * j + i) * BLOCK + group * PASSES;
+        if constexpr (PASSES == 2) {
+          *reinterpret_cast<uint16_t*>(to) = (uint16_t)pack4(x[0][i] * inv, x[1][i] * inv, 0.f, 0.f);
+        } else {
+#pragma unroll
+          for (int p = 0; p < PASSES; p += 4)
+            *reinterpret_cast<unsigned*>(to + p) = pack4(x[p][i] * inv, x[p + 1][i] * inv, x[p + 2][i] * inv, x[p + 3][i] * inv);
+        }
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // a wave's own bytes: nobody else to wait for
+    u32x4_t mine;  // which bytes of a coordinate's 16 are the run's
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       mine[w] = 0u;
@@ -217,7 +235,7 @@ __global__ __launch_bounds__(WAVE) void append8_kernel(Append a) {
     }
 #pragma unroll
     for (int d = lane; d < D; d += WAVE) {
-      u32x4_t* piece = reinterpret_cast<u32x4_t*>(at) + d;
+      u32x4_t* piece = reinterpret_cast<u32x4_t*>(base) + d;
       u32x4_t out = *reinterpret_cast<const u32x4_t*>(turned + d * BLOCK);
       if (n < BLOCK) {
         u32x4_t held = *piece;
@@ -228,8 +246,45 @@ __global__ __launch_bounds__(WAVE) void append8_kernel(Append a) {
       }
       *piece = out;
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
   if (lane == 0) scales[block] = scale;
+}
+
+template <int D, typename W> __global__ __launch_bounds__(256) void append8_kernel(Append a) {
+  constexpr int LPT = Lanes<D>::LPT;
+  __shared__ __align__(16) uint8_t turned[4][D * BLOCK];
+  const int lane = threadIdx.x & (WAVE - 1), j = lane % LPT, KV = a.pages.KV;
+  if ((int)blockIdx.x >= a.kv_blocks) {
+    append_query<D, W>(a, (blockIdx.x - a.kv_blocks) * (256 / LPT) + threadIdx.x / LPT, j);
+    return;
+  }
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), id = blockIdx.x * 4 + wave;
+  const int unit = id % (2 * KV), t0 = id / (2 * KV) * a.chunk;
+  if (t0 >= a.T) return;
+  const bool values = unit >= KV;
+  const int kvh = values ? unit - KV : unit;
+  // lane l looks at token t0 - 1 + l
+  const int t = t0 - 1 + lane;
+  const int slot = t >= 0 && t < a.T ? a.slots[t] : -2;
+  const int before = __shfl(slot, max(lane - 1, 0), WAVE);
+  const bool goes_on = slot > 0 && slot % BLOCK != 0 && before == slot - 1;  // in the run of the token before it
+  const unsigned long long on = __ballot(goes_on);
+  unsigned long long first = __ballot(lane >= 1 && lane <= a.chunk && slot >= 0 && slot / (a.pages.nb * BLOCK) < a.pages.num_pages && !goes_on);
+  float g[8];
+  const W* gains = (const W*)a.kw;
+  if (!values && gains && first) {
+    const Places at(8 * j < D ? j : 0, a.R);
+    load4(gains + at.a, g);
+    load4(gains + at.b, g + 4);
+  }
+  while (first) {  // uniform
+    const int l = __builtin_ctzll(first);
+    first &= first - 1;
+    const int n = __builtin_ctzll(~(on >> (l + 1))) + 1, s = __builtin_amdgcn_readlane(slot, l);
+    if (values) append_run<D, W, true>(a, t0 - 1 + l, n, s, kvh, g, turned[wave]);
+    else append_run<D, W, false>(a, t0 - 1 + l, n, s, kvh, g, turned[wave]);
+  }
 }
 
 // ---- attention --------------------------------------------------------------------------------------------
@@ -258,13 +313,9 @@ template <int D> __device__ __forceinline__ void load_query(Query<D>& q, const b
   for (int c = 0; c < D / 64; ++c)
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
-      float four[4];
-      load4(row + 64 * c + 16 * grp + i, four);
+      load4(row + 64 * c + 16 * grp + i, x[c] + i);
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        x[c][i + n] = four[n];
-        amax = fmaxf(amax, fabsf(four[n]));
-      }
+      for (int n = 0; n < 4; ++n) amax = fmaxf(amax, fabsf(x[c][i + n]));
     }
   q.scale = block_scale(quad_rows_max(amax));
   const float inv = inverse_of(q.scale);
@@ -941,14 +992,20 @@ extern "C" int as_qk_norm_rope_store8(const void* qkv, const void* qw, const voi
   if ((qw == nullptr) != (kw == nullptr) || !qkv || !q_out) return AS_BAD_SHAPE;
   if (store && (!slots || !pages_ok(k_pages, v_pages, k_scales, v_scales, num_pages, KV, D, bs))) return AS_BAD_SHAPE;
   if (w_dtype != DT_F32 && w_dtype != DT_BF16) return AS_BAD_DTYPE;
+  // A wave of keys and values takes the runs that start among 1, 4 or 16 tokens: few tokens' runs side by side, many tokens (of prompts: a run every
+  // sixteenth) without a wave for each.
+  int chunk = 1;
+  while (chunk < 16 && (long long)num_tokens * 2 * KV > 8192ll * chunk) chunk *= 4;
+  const long long kv_blocks = store ? (((long long)num_tokens + chunk - 1) / chunk * 2 * KV + 3) / 4 : 0;
   const Append a{(const bf16*)qkv, qw, kw, (const float2*)cs, slots, (bf16*)q_out,
-                 pages_of(k_pages, v_pages, k_scales, v_scales, num_pages, KV, bs), num_tokens, H, R, eps};
-#define LAUNCH(DV)                                                                          \
-  {                                                                                         \
-    constexpr int at_once = Lanes<DV>::AT_ONCE;                                             \
-    const dim3 grid(num_tokens, (H + at_once - 1) / at_once + (store ? 2 * KV : 0));        \
-    if (w_dtype == DT_F32) append8_kernel<DV, float><<<grid, WAVE, 0, stream>>>(a);         \
-    else append8_kernel<DV, bf16><<<grid, WAVE, 0, stream>>>(a);                            \
+                 pages_of(k_pages, v_pages, k_scales, v_scales, num_pages, KV, bs), num_tokens, H, R, eps, chunk, (int)kv_blocks};
+#define LAUNCH(DV)                                                                                       \
+  {                                                                                                      \
+    constexpr int groups = 256 / Lanes<DV>::LPT;                                                         \
+    const long long blocks = kv_blocks + ((long long)num_tokens * H + groups - 1) / groups;              \
+    if (blocks * groups > 0x7fffffffll) return AS_BAD_SHAPE;                                             \
+    if (w_dtype == DT_F32) append8_kernel<DV, float><<<(int)blocks, 256, 0, stream>>>(a);                \
+    else append8_kernel<DV, bf16><<<(int)blocks, 256, 0, stream>>>(a);                                   \
   }
   FOR_WIDTH(LAUNCH)
 #undef LAUNCH
