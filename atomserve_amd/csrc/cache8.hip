@@ -33,12 +33,12 @@ __device__ __forceinline__ float block_scale(float amax) {
 // 1 / 2^e, exact
 __device__ __forceinline__ float inverse_of(float scale) { return __uint_as_float((254u << 23) - __float_as_uint(scale)); }
 
-// Four numbers as e4m3, to the nearest, in a word.
+// Four numbers of at most 448 as e4m3, to the nearest, in a word.
 __device__ __forceinline__ unsigned pack4(float a, float b, float c, float d) {
-  auto in = [](float x) { return __builtin_amdgcn_fmed3f(x, -LARGEST, LARGEST); };
-  int r = __builtin_amdgcn_cvt_pk_fp8_f32(in(a), in(b), 0, false);
-  return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(in(c), in(d), r, true);
+  const int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
 }
+__device__ __forceinline__ float at_most_largest(float x) { return __builtin_amdgcn_fmed3f(x, -LARGEST, LARGEST); }
 __device__ __forceinline__ unsigned rescale4(unsigned w, float by) {
   const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
   return pack4(a[0] * by, a[1] * by, b[0] * by, b[1] * by);
@@ -59,7 +59,7 @@ __device__ __forceinline__ size_t block_index(const Pages& p, int page, int kvh,
 // are not turned; no lane needs another's but for the sum of squares.
 //
 // Queries: a group of lanes a (token, head), heads side by side.  Keys and values: a wave takes the runs that start among `chunk` neighbouring tokens, for
-// one kv head's keys or values.  A run: tokens next to each other in the step that go to places next to each other of one block, so that one wave sees
+// one kv head's keys or values; single tokens several at once, longer runs one after the other.  A run: tokens next to each other in the step that go to places next to each other of one block, so that one wave sees
 // all that the step puts there: the largest magnitude, the scale, and what the block held.  Lane group s has the run's places PASSES s .. + PASSES - 1 of the
 // block, so that a coordinate's bytes are neighbours in a lane's hands: they cross to the transposed block through LDS.
 template <int D> struct Lanes {
@@ -73,6 +73,17 @@ template <int LPT> __device__ __forceinline__ float lanes_sum(float v) {
   v += dpp<DPP_XOR_1>(v);
   v += dpp<DPP_XOR_2>(v);
   return v + dpp<DPP_HALF_MIRROR>(v);
+}
+
+template <int LPT> __device__ __forceinline__ float lanes_max(float v) {
+  if constexpr (LPT >= 32) {
+    const TwoHalves h = halves_16(v);
+    v = fmaxf(h.a, h.b);
+  }
+  if constexpr (LPT >= 16) v = fmaxf(v, dpp<DPP_ROTATE(8)>(v));
+  v = fmaxf(v, dpp<DPP_XOR_1>(v));
+  v = fmaxf(v, dpp<DPP_XOR_2>(v));
+  return fmaxf(v, dpp<DPP_HALF_MIRROR>(v));
 }
 
 __device__ __forceinline__ void load4(const bf16* p, float* x) {
@@ -108,20 +119,25 @@ struct Places {
   }
 };
 
-// Norm (gains g, or none) and rotation of a head's eight coordinates in this lane by the angles of token t.
+// Norm (gains g, or none) and rotation of a head's eight coordinates in this lane by the angles of token t.  busy: the lane has coordinates of its own.
 template <int D>
-__device__ __forceinline__ void norm_turn(float (&x)[8], bool norm, const float (&g)[8], const float2* cs, float eps, int R, int t, int j) {
+__device__ __forceinline__ void norm_turn(float (&x)[8], bool norm, const float (&g)[8], const float2* cs, float eps, int R, int t, int j, bool busy) {
+  const bool turns = busy && 8 * j < R;
+  float4 a, b;
+  if (turns) {
+    const float4* angles = reinterpret_cast<const float4*>(cs + (size_t)t * (R / 2) + 4 * j);
+    a = angles[0];
+    b = angles[1];
+  }
   if (norm) {
     float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss += x[i] * x[i];  // 0 in lanes without coordinates
-    const float inv = 1.0f / sqrtf(lanes_sum<Lanes<D>::LPT>(ss) / (float)D + eps);
+    for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+    const float inv = __builtin_amdgcn_rsqf(lanes_sum<Lanes<D>::LPT>(D == 192 && !busy ? 0.f : ss) * (1.f / (float)D) + eps);  // to one step of fp32
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * g[i];
   }
-  if (8 * j < R) {
-    const float4* angles = reinterpret_cast<const float4*>(cs + (size_t)t * (R / 2) + 4 * j);
-    const float4 a = angles[0], b = angles[1];
+  if (turns) {
     const float c[4] = {a.x, a.z, b.x, b.z}, s[4] = {a.y, a.w, b.y, b.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -138,16 +154,14 @@ template <int D, typename W> __device__ __forceinline__ void append_query(const 
   const bool busy = 8 * j < D;
   const Places at(busy ? j : 0, a.R);
   const bf16* src = a.qkv + ((size_t)t * (a.H + 2 * a.pages.KV) + h) * D;
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, g[8];
-  if (busy) {
-    load4(src + at.a, x);
-    load4(src + at.b, x + 4);
-  }
+  float x[8], g[8];
+  load4(src + at.a, x);
+  load4(src + at.b, x + 4);
   if (a.qw) {
     load4((const W*)a.qw + at.a, g);
     load4((const W*)a.qw + at.b, g + 4);
   }
-  norm_turn<D>(x, a.qw != nullptr, g, a.cs, a.eps, busy ? a.R : 0, t, j);
+  norm_turn<D>(x, a.qw != nullptr, g, a.cs, a.eps, a.R, t, j, busy);
   if (!busy) return;
   bf16* dst = a.q_out + ((size_t)t * a.H + h) * D;
   *reinterpret_cast<bf16x4_t*>(dst + at.a) = bf16x4_t{(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]};
@@ -164,36 +178,48 @@ __device__ __forceinline__ void append_run(const Append& a, int t, int n, int sl
   const Places at(busy ? j : 0, R);
   const size_t block = block_index(a.pages, slot / bs, kvh, slot % bs / BLOCK);
   const bf16* src = a.qkv + ((size_t)t * heads + a.H + (VALUES ? a.pages.KV : 0) + kvh) * D;
-  float x[PASSES][8], amax = 0.f;
-#pragma unroll
-  for (int p = 0; p < PASSES; ++p) {
-    const int nth = group * PASSES + p - off;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[p][i] = 0.f;
-    if (busy && nth >= 0 && nth < n) {
-      load4(src + (size_t)nth * heads * D + at.a, x[p]);
-      load4(src + (size_t)nth * heads * D + at.b, x[p] + 4);
-    }
-  }
-#pragma unroll
-  for (int p = 0; p < PASSES; ++p) {
-    const int nth = group * PASSES + p - off;
-    if constexpr (!VALUES) {
-      if (__any(nth >= 0 && nth < n)) norm_turn<D>(x[p], a.kw != nullptr, g, a.cs, a.eps, busy ? R : 0, t + min(max(nth, 0), n - 1), j);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[p][i] = finite_or_zero(x[p][i]);
-      amax = fmaxf(amax, fabsf(x[p][i]));
-    }
-  }
-  amax = wave_max(amax);
   float* scales = VALUES ? a.pages.vs : a.pages.ks;
+  uint8_t* base = (VALUES ? a.pages.v : a.pages.k) + block * (BLOCK * D);
+  // All that is read is asked for before anything is waited for.  Places that are not the run's repeat one of its tokens: nothing to choose between
+  // but where results are stored.
+  float x[PASSES][8];
+  u32x4_t held[D / 64];
   const float before = off > 0 ? scales[block] : 0.f;  // a block that begins with this run is new
+  if constexpr (VALUES) {
+    if (n < BLOCK) {
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) held[i] = reinterpret_cast<const u32x4_t*>(base)[64 * i + lane];
+    }
+  }
+  auto nth = [&](int p) { return min(max(group * PASSES + p - off, 0), n - 1); };
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    const bf16* from = src + (size_t)nth(p) * heads * D;
+    load4(from + at.a, x[p]);
+    load4(from + at.b, x[p] + 4);
+  }
+  unsigned most = 0;  // the largest magnitude's bits
+#pragma unroll
+  for (int p = 0; p < PASSES; ++p) {
+    if constexpr (!VALUES) norm_turn<D>(x[p], a.kw != nullptr, g, a.cs, a.eps, R, t + nth(p), j, busy);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[p][i]) & 0x7fffffffu);
+  }
+  float amax = wave_max(__uint_as_float(min(most, 0x7f800000u)));
+  if (amax > LARGEST * 0x1p119f) {  // uniform, and rare: numbers that are not finite are zeros, and larger ones the largest that a scale reaches
+    most = 0;
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[p][i] = __builtin_amdgcn_fmed3f(finite_or_zero(x[p][i]), -LARGEST * 0x1p119f, LARGEST * 0x1p119f);
+        most = max(most, __float_as_uint(x[p][i]) & 0x7fffffffu);
+      }
+    amax = wave_max(__uint_as_float(most));
+  }
   const float scale = fmaxf(before, block_scale(amax)), inv = inverse_of(scale);
   const bool grows = before > 0.f && scale > before;
   const float by = before * inv;
-  uint8_t* base = (VALUES ? a.pages.v : a.pages.k) + block * (BLOCK * D);
   if constexpr (!VALUES) {
     if (grows) {  // the block's other rows at the new scale
       for (int w = lane; w < BLOCK * D / 4; w += WAVE) {
@@ -234,21 +260,92 @@ __device__ __forceinline__ void append_run(const Append& a, int t, int n, int sl
         if (4 * w + b >= off && 4 * w + b < off + n) mine[w] |= 0xffu << (8 * b);
     }
 #pragma unroll
-    for (int d = lane; d < D; d += WAVE) {
-      u32x4_t* piece = reinterpret_cast<u32x4_t*>(base) + d;
-      u32x4_t out = *reinterpret_cast<const u32x4_t*>(turned + d * BLOCK);
+    for (int i = 0; i < D / 64; ++i) {
+      u32x4_t out = *reinterpret_cast<const u32x4_t*>(turned + (64 * i + lane) * BLOCK);
       if (n < BLOCK) {
-        u32x4_t held = *piece;
         if (grows)
 #pragma unroll
-          for (int w = 0; w < 4; ++w) held[w] = rescale4(held[w], by);
-        out = (out & mine) | (held & ~mine);
+          for (int w = 0; w < 4; ++w) held[i][w] = rescale4(held[i][w], by);
+        out = (out & mine) | (held[i] & ~mine);
       }
-      *piece = out;
+      reinterpret_cast<u32x4_t*>(base)[64 * i + lane] = out;
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
   if (lane == 0) scales[block] = scale;
+}
+
+// Single tokens (decode steps), as many as a wave has groups of lanes, each group one: `tokens` has the lanes that look at them, `slot` what lane l looks at.
+// Nothing crosses lanes: a key is a row, a value a byte of every coordinate's 16, and only a scale that grows makes the rest of the block be read.
+template <int D, typename W, bool VALUES>
+__device__ __forceinline__ void append_singles(const Append& a, int t0, unsigned long long& tokens, int slot, int kvh, const float (&g)[8]) {
+  constexpr int LPT = Lanes<D>::LPT, AT_ONCE = Lanes<D>::AT_ONCE;
+  const int lane = threadIdx.x & (WAVE - 1), group = lane / LPT, j = lane % LPT, heads = a.H + 2 * a.pages.KV, bs = a.pages.nb * BLOCK;
+  const bool busy = 8 * j < D;
+  const int R = VALUES ? 0 : a.R;
+  const Places at(busy ? j : 0, R);
+  int t = -1, s = 0;
+#pragma unroll
+  for (int i = 0; i < AT_ONCE; ++i) {
+    if (!tokens) break;  // uniform
+    const int l = __builtin_ctzll(tokens), here = __builtin_amdgcn_readlane(slot, l);
+    tokens &= tokens - 1;
+    if (group >= i) {  // groups beyond the last token repeat it and store nothing
+      t = group == i ? t0 - 1 + l : -1;
+      s = here;
+    }
+  }
+  const bool mine = t >= 0;
+  if (!mine) return;  // whole groups leave
+  const int off = s % BLOCK;
+  const size_t block = block_index(a.pages, s / bs, kvh, s % bs / BLOCK);
+  float* scales = VALUES ? a.pages.vs : a.pages.ks;
+  uint8_t* base = (VALUES ? a.pages.v : a.pages.k) + block * (BLOCK * D);
+  const bf16* src = a.qkv + ((size_t)t * heads + a.H + (VALUES ? a.pages.KV : 0) + kvh) * D;
+  const float before = off > 0 ? scales[block] : 0.f;  // a block that begins with this token is new
+  float x[8];
+  load4(src + at.a, x);
+  load4(src + at.b, x + 4);
+  if constexpr (!VALUES) norm_turn<D>(x, a.kw != nullptr, g, a.cs, a.eps, R, t, j, busy);
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x[i] = __builtin_amdgcn_fmed3f(finite_or_zero(x[i]), -LARGEST * 0x1p119f, LARGEST * 0x1p119f);
+    amax = fmaxf(amax, fabsf(x[i]));
+  }
+  const float scale = fmaxf(before, block_scale(lanes_max<LPT>(amax))), inv = inverse_of(scale), by = before * inv;
+  const bool grows = before > 0.f && scale > before;
+  const unsigned lower = pack4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv), upper = pack4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
+  if constexpr (!VALUES) {
+    if (grows)  // the block's other rows at the new scale
+      for (int w = j; w < BLOCK * D / 4; w += LPT) {
+        unsigned* word = reinterpret_cast<unsigned*>(base) + w;
+        if (4 * w / D != off) *word = rescale4(*word, by);
+      }
+    if (busy) {
+      *reinterpret_cast<unsigned*>(base + off * D + at.a) = lower;
+      *reinterpret_cast<unsigned*>(base + off * D + at.b) = upper;
+    }
+  } else if (busy) {
+    const unsigned shift = 8 * (off & 3);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const unsigned byte = (i < 4 ? lower : upper) >> (8 * (i & 3)) & 0xffu;
+      uint8_t* piece = base + (8 * j + i) * BLOCK;
+      if (grows) {
+        u32x4_t held = *reinterpret_cast<const u32x4_t*>(piece);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          held[w] = rescale4(held[w], by);
+          if (off >> 2 == w) held[w] = (held[w] & ~(0xffu << shift)) | byte << shift;
+        }
+        *reinterpret_cast<u32x4_t*>(piece) = held;
+      } else {
+        piece[off] = (uint8_t)byte;
+      }
+    }
+  }
+  if (j == 0) scales[block] = scale;
 }
 
 template <int D, typename W> __global__ __launch_bounds__(256) void append8_kernel(Append a) {
@@ -259,8 +356,8 @@ template <int D, typename W> __global__ __launch_bounds__(256) void append8_kern
     append_query<D, W>(a, (blockIdx.x - a.kv_blocks) * (256 / LPT) + threadIdx.x / LPT, j);
     return;
   }
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), id = blockIdx.x * 4 + wave;
-  const int unit = id % (2 * KV), t0 = id / (2 * KV) * a.chunk;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int id = blockIdx.x * 4 + wave, unit = id % (2 * KV), t0 = id / (2 * KV) * a.chunk;
   if (t0 >= a.T) return;
   const bool values = unit >= KV;
   const int kvh = values ? unit - KV : unit;
@@ -278,9 +375,15 @@ template <int D, typename W> __global__ __launch_bounds__(256) void append8_kern
     load4(gains + at.a, g);
     load4(gains + at.b, g + 4);
   }
-  while (first) {  // uniform
-    const int l = __builtin_ctzll(first);
-    first &= first - 1;
+  // first: the lanes whose tokens begin a run of this wave's; a run of one has nobody that goes on behind it
+  unsigned long long singles = first & ~(on >> 1), runs = first & on >> 1;
+  while (singles) {  // uniform
+    if (values) append_singles<D, W, true>(a, t0, singles, slot, kvh, g);
+    else append_singles<D, W, false>(a, t0, singles, slot, kvh, g);
+  }
+  while (runs) {
+    const int l = __builtin_ctzll(runs);
+    runs &= runs - 1;
     const int n = __builtin_ctzll(~(on >> (l + 1))) + 1, s = __builtin_amdgcn_readlane(slot, l);
     if (values) append_run<D, W, true>(a, t0 - 1 + l, n, s, kvh, g, turned[wave]);
     else append_run<D, W, false>(a, t0 - 1 + l, n, s, kvh, g, turned[wave]);
@@ -325,7 +428,7 @@ template <int D> __device__ __forceinline__ void load_query(Query<D>& q, const b
     for (int w = 0; w < 4; ++w) {
       float y[4];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) y[n] = x[c][4 * w + n] * inv;
+      for (int n = 0; n < 4; ++n) y[n] = at_most_largest(x[c][4 * w + n] * inv);
       const unsigned high = pack4(y[0], y[1], y[2], y[3]);
       const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)high, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)high, true);
       q.high[c][w] = high;
@@ -992,13 +1095,11 @@ extern "C" int as_qk_norm_rope_store8(const void* qkv, const void* qw, const voi
   if ((qw == nullptr) != (kw == nullptr) || !qkv || !q_out) return AS_BAD_SHAPE;
   if (store && (!slots || !pages_ok(k_pages, v_pages, k_scales, v_scales, num_pages, KV, D, bs))) return AS_BAD_SHAPE;
   if (w_dtype != DT_F32 && w_dtype != DT_BF16) return AS_BAD_DTYPE;
-  // A wave of keys and values takes the runs that start among 1, 4 or 16 tokens: few tokens' runs side by side, many tokens (of prompts: a run every
-  // sixteenth) without a wave for each.
-  int chunk = 1;
-  while (chunk < 16 && (long long)num_tokens * 2 * KV > 8192ll * chunk) chunk *= 4;
+  if (R == 0) cs = nullptr;
+  const int chunk = (long long)num_tokens * KV <= 2048 ? 4 : 16;
   const long long kv_blocks = store ? (((long long)num_tokens + chunk - 1) / chunk * 2 * KV + 3) / 4 : 0;
-  const Append a{(const bf16*)qkv, qw, kw, (const float2*)cs, slots, (bf16*)q_out,
-                 pages_of(k_pages, v_pages, k_scales, v_scales, num_pages, KV, bs), num_tokens, H, R, eps, chunk, (int)kv_blocks};
+  const Append a{(const bf16*)qkv, qw, kw, (const float2*)cs, slots, (bf16*)q_out, pages_of(k_pages, v_pages, k_scales, v_scales, num_pages, KV, bs),
+           num_tokens, H, R, eps, chunk, (int)kv_blocks};
 #define LAUNCH(DV)                                                                                       \
   {                                                                                                      \
     constexpr int groups = 256 / Lanes<DV>::LPT;                                                         \
