@@ -914,6 +914,49 @@ def attn_single_query8(q, k_pages, v_pages, k_scales, v_scales, items, positions
          float(scale), *sight, part_size, P, share, _stream())  # fmt: skip
 
 
+# What a step of portions over 8 bits costs, in microseconds fitted to the kernel's times of 435 steps (1 to 16 portions of 9 to 2,048 tokens behind 0 to
+# 30,000; 16 to 64 heads of 64, 128, 192 and 256; 256 compute units), by (column tiles of 16 queries that a wave owns, head width): a round of 64 keys where a
+# workgroup has a compute unit to itself, a round where all places are taken, and the places.  Workgroups are counted as far as items are long enough to be
+# cut; items of every length (spread 1: a lone prompt) share their places less, and more workgroups than places last for all the work divided by the places and a
+# fifth of a piece, or whole turns as far as items are equally long.  What it picks takes 4 per cent more than the best of 16 forms on average and 54 at worst (the rule of
+# 16-bit pages, `_prefill_plan`, 8 and 106; for heads of 192, whose 32 queries a wave leave room for one workgroup, 6 and 32).
+PREFILL8_ROUNDS = {(1, 64): (0.70, 1.48, 4), (2, 64): (1.17, 2.07, 3), (1, 128): (0.89, 1.57, 3), (2, 128): (1.46, 2.09, 2), (1, 192): (1.45, 1.94, 2),
+                   (2, 192): (2.34, 2.76, 1), (1, 256): (1.65, 1.95, 1), (2, 256): (3.04, 3.42, 1)}  # fmt: skip
+PREFILL8_PIECES = (1, 2, 3, 4, 6, 8, 12, 16)
+PREFILL8_MIN_PIECE_ROUNDS = 4
+
+
+def _prefill8_cost(num_tiles, H, KV, D, rounds, mean_rounds, query_tiles, pieces) -> float:
+    alone, shared, per_unit = PREFILL8_ROUNDS[query_tiles, D]
+    units, piece = compute_units(), -(-rounds // pieces)
+    spread = min(1.0, max(0.0, 2.0 * (1.0 - mean_rounds / rounds)))
+    workgroups = num_tiles * KV * _prefill_units(query_tiles, H // KV) * min(pieces, max(1.0, mean_rounds / piece + 0.5 * spread))
+    places = per_unit * units
+    if workgroups <= units:
+        cost = piece * alone
+    elif workgroups <= places:
+        cost = piece * (alone + (shared - alone) * (workgroups - units) / (places - units) * (1.0 - 0.55 * spread))
+    else:
+        work = num_tiles * KV * (64 // (16 * query_tiles)) * (H // KV) / 4 * mean_rounds  # rounds of full workgroups
+        evenly = max(piece * alone, (work / places + 0.2 * piece) * shared)
+        cost = spread * evenly + (1.0 - spread) * math.ceil(workgroups / places) * piece * shared
+    return cost + (6.7 + 64 * num_tiles * H * pieces * D * 8 / 9.7e6 if pieces > 1 else 0.0)
+
+
+@functools.lru_cache(maxsize=1024)
+def _prefill8_plan(num_tiles, H, KV, D, max_context, window, query_tiles, tile_keys, forced_pieces, units, keep_first=0) -> tuple:
+    """(query tiles of a wave, pieces, rounds of a piece) for a step of portions over 8 bits; pieces 1 (and 0 rounds): nothing is cut.  Asked once a
+    step: every layer's question is the same."""
+    rounds, mean_rounds = _prefill_rounds(num_tiles, max_context, window, tile_keys, keep_first)
+    kinds = (2, 1) if query_tiles is None else (int(query_tiles),)
+    if forced_pieces is not None:
+        cuts = (max(1, min(int(forced_pieces), rounds // 2)),)
+    else:
+        cuts = tuple(c for c in PREFILL8_PIECES if c == 1 or rounds // c >= PREFILL8_MIN_PIECE_ROUNDS)
+    kind, pieces = min(((k, c) for k in kinds for c in cuts), key=lambda kc: _prefill8_cost(num_tiles, H, KV, D, rounds, mean_rounds, *kc))
+    return (kind, pieces, -(-rounds // pieces)) if pieces > 1 else (kind, 1, 0)
+
+
 def attn_prefill8(q, k_pages, v_pages, k_scales, v_scales, tiles, block_tables, out, scale, window, max_context, query_tiles=None,
                   tile_keys: int = 0, keep_first=0, softcap=0.0, sink=False, chunk=0) -> None:  # fmt: skip
     """`attn_prefill` over a cache in 8 bits: arguments as there."""
@@ -931,7 +974,8 @@ def attn_prefill8(q, k_pages, v_pages, k_scales, v_scales, tiles, block_tables, 
         raise KernelError("attention over 8 bits: scores have a positive scale")
     if max_context > block_tables.shape[1] * bs:
         raise KernelError("attention: block tables are shorter than the longest context")
-    query_tiles, pieces, piece_rounds = _prefill_plan(tiles.shape[0], H, KV, D, max_context, window or chunk, query_tiles, tile_keys, sight[1])
+    query_tiles, pieces, piece_rounds = _prefill8_plan(tiles.shape[0], H, KV, D, max_context, window or chunk, query_tiles or PREFILL_QUERY_TILES,
+                                                       tile_keys, PREFILL_PIECES, compute_units(), sight[1])  # fmt: skip
     cut = part_ml = part_acc = None
     if pieces > 1:
         cut = torch.empty(tiles.shape[0] * KV * _prefill_units(query_tiles, H // KV), dtype=I32, device=q.device)

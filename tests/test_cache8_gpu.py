@@ -321,10 +321,10 @@ def test_prompts_masks(ops, kw):
 def test_prompts_cut_along_their_keys(ops, monkeypatch, query_tiles, pieces, kw):
     """Items of every length in a step that is cut: the short ones stay whole."""
     monkeypatch.setattr(ops, "PREFILL_PIECES", pieces)
-    ops._prefill_plan_of.cache_clear()
+    ops._prefill8_plan.cache_clear()
     prompt(ops, 6, 2, 64, 32, [(100, 1500), (70, 0), (5, 700), (64, 192)], query_tiles=query_tiles, **kw)
     prompt(ops, 10, 2, 128, 16, [(65, 1100), (40, 20)], query_tiles=query_tiles, **kw)
-    ops._prefill_plan_of.cache_clear()
+    ops._prefill8_plan.cache_clear()
 
 
 def test_prompts_longer(ops):
