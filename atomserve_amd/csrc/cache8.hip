@@ -1138,11 +1138,11 @@ extern "C" int as_qk_norm_rope_store8(const void* qkv, const void* qw, const voi
   return launch_status();
 }
 
-// Single queries.  part_m, part_l [N, H, P], part_acc [N, H, P, D] fp32 where P > 1; part_size: keys of a partition, a multiple of 64; share: how
+// Single queries.  parts: fp32 [N, H, P, D + 2] where P > 1, unnormalised outputs, then maxima, then sums; part_size: keys of a partition, a multiple of 64; share: how
 // many of the KV groups of query heads (at most 16 to a group) read one head of the pages, which hold KV / share.
 extern "C" int as_attn_single_query8(const void* q, const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
                                      int num_pages, const int* items, int num_items, const int* positions, const int* tok_row,
-                                     const int* block_tables, int table_width, void* out, float* part_m, float* part_l, float* part_acc, int H,
+                                     const int* block_tables, int table_width, void* out, float* parts, int H,
                                      int KV, int D, int bs, float scale, int window, int keep, int chunk, float cap, int sink,
                                      const float* sinks, int wide, int part_size, int P, int share, hipStream_t stream) {
   if (num_items <= 0) return AS_OK;
@@ -1150,9 +1150,11 @@ extern "C" int as_attn_single_query8(const void* q, const void* k_pages, const v
   if (!sight_ok(sight) || H <= 0 || KV <= 0 || H % KV || H / KV > 16 || share < 1 || KV % share) return AS_BAD_SHAPE;
   if (!pages_ok(k_pages, v_pages, k_scales, v_scales, num_pages, KV / share, D, bs) || !table_ok(num_pages, KV / share, bs, table_width)) return AS_BAD_SHAPE;
   if (!q || !positions || !block_tables || !out || part_size <= 0 || part_size % STEP || P <= 0 || P > 65535 || num_items > 65535) return AS_BAD_SHAPE;
-  if (P > 1 && (!part_m || !part_l || !part_acc)) return AS_BAD_SHAPE;
+  if (P > 1 && (!parts || (uintptr_t)parts & 15)) return AS_BAD_SHAPE;
+  const size_t rows = P > 1 ? (size_t)num_items * H * P : 0;
   const Attend a{(const bf16*)q, pages_of(k_pages, v_pages, k_scales, v_scales, num_pages, KV / share, bs), items, positions, tok_row, nullptr,
-                 block_tables, table_width, (bf16*)out, part_m, part_l, part_acc, H, KV, share, scale, sight, part_size / STEP, P, magic_of(bs), compute_units()};
+                 block_tables, table_width, (bf16*)out, parts + rows * D, parts + rows * (D + 1), parts, H, KV, share, scale, sight, part_size / STEP, P,
+                 magic_of(bs), compute_units()};
   const size_t shmem = sizeof(float) * (128 + 4 * (size_t)(D + 4) * (H / KV));
 #define LAUNCH(DV)                                                                                                                       \
   {                                                                                                                                      \
@@ -1170,26 +1172,27 @@ extern "C" int as_attn_single_query8(const void* q, const void* k_pages, const v
 
 // Portions of prompts: tiles [num_tiles, 4] int32 (first token, count <= 64, row of block_tables, position of the first), best those that see most keys
 // first.  query_tiles: 2, a wave owns 32 queries of a head; 1, 16 (twice the workgroups).  pieces > 1: items of more than piece_rounds rounds of 64 keys
-// are cut; cut [num_tiles * KV * ceil(64 / (16 query_tiles) * (H / KV) / 4)] int32, part_ml [T, H, pieces, 2] and part_acc [T, H, pieces, D] fp32 with T one
-// more than the largest token of a tile; piece_rounds * pieces covers the longest item.  pieces <= 1: none is cut, the three may be null.
+// are cut; parts: 32-bit words, [T, H, pieces, D] unnormalised outputs, [T, H, pieces, 2] maxima and sums and [num_tiles * KV * ceil(64 / (16 query_tiles) *
+// (H / KV) / 4)] integers, with T (`tokens`) one more than the largest token of a tile; piece_rounds * pieces covers the longest item.  pieces <= 1: none is
+// cut, parts may be null.
 extern "C" int as_attn_prefill8(const void* q, const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
                                 int num_pages, const int* tiles, int num_tiles, const int* block_tables, int table_width, void* out, int H,
                                 int KV, int D, int bs, float scale, int window, int keep, int chunk, float cap, int sink, const float* sinks,
-                                int wide, int query_tiles, int pieces, int piece_rounds, int* cut, float* part_ml, float* part_acc,
-                                hipStream_t stream) {
+                                int wide, int query_tiles, int pieces, int piece_rounds, float* parts, int tokens, hipStream_t stream) {
   if (num_tiles <= 0) return AS_OK;
   const Sight sight{window, keep, chunk, cap, sink, sinks, wide};
   if (!sight_ok(sight) || H <= 0 || KV <= 0 || H % KV || (query_tiles != 1 && query_tiles != 2)) return AS_BAD_SHAPE;
   if (!pages_ok(k_pages, v_pages, k_scales, v_scales, num_pages, KV, D, bs) || !table_ok(num_pages, KV, bs, table_width)) return AS_BAD_SHAPE;
   if (!q || !tiles || !block_tables || !out) return AS_BAD_SHAPE;
   if (pieces < 1) pieces = 1;
-  if (pieces > 1 && (piece_rounds < 1 || !cut || !part_ml || !part_acc)) return AS_BAD_SHAPE;
+  if (pieces > 1 && (piece_rounds < 1 || !parts || (uintptr_t)parts & 15 || tokens <= 0)) return AS_BAD_SHAPE;
   const int units_z = (64 / (16 * query_tiles) * (H / KV) + 3) / 4;
   const long long items = (long long)num_tiles * KV * units_z;
   if (items * pieces > 0x7fffffffll) return AS_BAD_SHAPE;
   const Attend a{(const bf16*)q, pages_of(k_pages, v_pages, k_scales, v_scales, num_pages, KV, bs), nullptr, nullptr, nullptr, tiles, block_tables,
                  table_width, (bf16*)out, nullptr, nullptr, nullptr, H, KV, 1, scale, sight, 0, 1, magic_of(bs), compute_units()};
-  const Cut how{pieces, piece_rounds, cut, part_ml, part_acc};
+  const size_t rows = pieces > 1 ? (size_t)tokens * H * pieces : 0;
+  const Cut how{pieces, piece_rounds, (int*)(parts + rows * (D + 2)), parts + rows * D, parts};
 #define LAUNCH2(DV, QTV)                                                                                           \
   {                                                                                                                \
     prompt8_kernel<DV, QTV><<<(int)(items * pieces), 256, 0, stream>>>(a, units_z, compute_units(), how);          \

@@ -859,23 +859,45 @@ def _up64(n: int) -> int:
     return -(-n // STEP8) * STEP8
 
 
+# What single queries over 8 bits cost, in microseconds fitted to the kernel's times of 240 sets of up to 64 requests of 100 to 131,072 keys (16 to 64 heads of
+# 128 on 8 kv heads, 28 heads of 64 on 4, 8 heads on 1 and 4; 256 compute units), by head width: a workgroup, a key of it (four waves, 256 keys at a time),
+# and how many workgroups a compute unit has at once.  A step lasts as long as a workgroup, or as all of them take their places, and no less than memory
+# (7.3 TB/s) needs; the merge is 1.6 us, 0.04 a partition and 2.3 TB/s for what partitions leave.  From one and a half (token, kv head) pairs a compute
+# unit on contexts stay whole, which many requests of unequal length want.  What it picks takes 1.3 per cent more than the best of eight sizes on
+# average and 20 at worst (the rule of 16-bit pages, 4.5 and 54).
+SINGLE8_COSTS = {64: (4.1, 0.0033, 4.4), 128: (4.7, 0.0055, 2.66), 192: (5.2, 0.0084, 1.1), 256: (5.7, 0.0113, 1.1)}
+SINGLE8_PARTITIONS = (128, 256, 512, 1024, 2048, 4096, 8192)
+
+
+@functools.lru_cache(maxsize=1024)
+def _partition8(N: int, H: int, KV: int, D: int, span: int, units: int) -> int:
+    """Keys of a partition for N single queries that see up to `span` keys (a multiple of 64)."""
+    groups = N * KV
+    if groups >= units * 3 // 2:
+        return span
+    start, key, per_unit = SINGLE8_COSTS[D]
+    memory = groups * span * 2 * D / 7.3e6 + start
+
+    def cost(part: int) -> float:
+        one, parts = start + key * part, span / part
+        busy = max(one, groups * (start * max(1.0, parts) + key * span) / (per_unit * units))
+        merge = 1.6 + 0.04 * math.ceil(parts) + N * H * math.ceil(parts) * D * 8 / 2.3e6 if part < span else 0.0
+        return (busy**4 + memory**4) ** 0.25 + merge
+
+    return min((span, *(part for part in SINGLE8_PARTITIONS if part < span)), key=cost)
+
+
 def _partitions8(N, H, KV, D, max_context, window, part_size, device, keep_first=0):
     """`_partitions` for the kernel of single queries over 8 bits, whose steps are 64 keys."""
     span = _up64(max_context) if window <= 0 else min(_up64(max_context), _up64(window + STEP8 - 1) + _up64(keep_first))
     if part_size is None:
-        if N * KV >= attn_fill_groups():
-            part_size = span
-        else:
-            part_size = min(MFMA_PARTITIONS, key=lambda part: _partition_cost(N * KV, span, part) + (MERGE_LAUNCH if part < span else 0.0))
+        part_size = _partition8(N, H, KV, D, span, compute_units())
     if part_size <= 0 or part_size % STEP8:
         raise KernelError(f"attention over 8 bits: partitions are multiples of {STEP8} keys")
     P = max(1, math.ceil(span / part_size))
-    part_m = part_l = part_acc = None
-    if P > 1:
-        part_m = torch.empty((N, H, P), dtype=F32, device=device)
-        part_l = torch.empty((N, H, P), dtype=F32, device=device)
-        part_acc = torch.empty((N, H, P, D), dtype=F32, device=device)
-    return part_size, P, part_m, part_l, part_acc
+    if P == 1:
+        return part_size, 1, None
+    return part_size, P, torch.empty(N * H * P * (D + 2), dtype=F32, device=device)
 
 
 def _share8(group: int) -> int:
@@ -908,9 +930,9 @@ def attn_single_query8(q, k_pages, v_pages, k_scales, v_scales, items, positions
     if max_context > block_tables.shape[1] * bs:
         raise KernelError("attention: block tables are shorter than the longest context")
     share = _share8(H // KV)
-    part_size, P, part_m, part_l, part_acc = _partitions8(N, H, KV * share, D, max_context, window or chunk, part_size, q.device, sight[1])
+    part_size, P, parts = _partitions8(N, H, KV * share, D, max_context, window or chunk, part_size, q.device, sight[1])
     call("as_attn_single_query8", _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales), NB, _ptr(items), N, _ptr(positions),
-         _ptr(tok_row), _ptr(block_tables), block_tables.shape[1], _ptr(out), _ptr(part_m), _ptr(part_l), _ptr(part_acc), H, KV * share, D, bs,
+         _ptr(tok_row), _ptr(block_tables), block_tables.shape[1], _ptr(out), _ptr(parts), H, KV * share, D, bs,
          float(scale), *sight, part_size, P, share, _stream())  # fmt: skip
 
 
@@ -976,14 +998,12 @@ def attn_prefill8(q, k_pages, v_pages, k_scales, v_scales, tiles, block_tables, 
         raise KernelError("attention: block tables are shorter than the longest context")
     query_tiles, pieces, piece_rounds = _prefill8_plan(tiles.shape[0], H, KV, D, max_context, window or chunk, query_tiles or PREFILL_QUERY_TILES,
                                                        tile_keys, PREFILL_PIECES, compute_units(), sight[1])  # fmt: skip
-    cut = part_ml = part_acc = None
+    parts = None  # outputs, maxima and sums of the pieces, and how many pieces each item has
     if pieces > 1:
-        cut = torch.empty(tiles.shape[0] * KV * _prefill_units(query_tiles, H // KV), dtype=I32, device=q.device)
-        part_ml = torch.empty((T, H, pieces, 2), dtype=F32, device=q.device)
-        part_acc = torch.empty((T, H, pieces, D), dtype=F32, device=q.device)
+        parts = torch.empty(T * H * pieces * (D + 2) + tiles.shape[0] * KV * _prefill_units(query_tiles, H // KV), dtype=F32, device=q.device)
     call("as_attn_prefill8", _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales), NB, _ptr(tiles), tiles.shape[0],
-         _ptr(block_tables), block_tables.shape[1], _ptr(out), H, KV, D, bs, float(scale), *sight, int(query_tiles), pieces, piece_rounds, _ptr(cut),
-         _ptr(part_ml), _ptr(part_acc), _stream())  # fmt: skip
+         _ptr(block_tables), block_tables.shape[1], _ptr(out), H, KV, D, bs, float(scale), *sight, int(query_tiles), pieces, piece_rounds, _ptr(parts), T,
+         _stream())  # fmt: skip
 
 
 SKINNY_MAX_ROWS = 16  # up to here the bf16 product streams the weights through our own kernel
