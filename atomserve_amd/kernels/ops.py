@@ -808,16 +808,45 @@ def cache8_supported(dtype, num_heads: int, num_kv_heads: int, head_dim: int, bl
             and rotary_dim % 8 == 0)  # fmt: skip
 
 
-def _check_pages8(k_pages, v_pages, k_scales, v_scales, num_kv_heads=None) -> tuple:
+# The calls below are made once a layer and are as long as their Python where steps are not replayed: one expression per call looks at all that is usually
+# right, and `_check` says what is wrong where it is not (append of one token, host and launch: 14.5 us with a check per tensor).
+
+
+def _good(t, dtype, shape) -> bool:
+    return t.dtype is dtype and t.shape == shape and t.is_cuda and t.is_contiguous()
+
+
+def _pages8(k_pages, v_pages, k_scales, v_scales, num_kv_heads=None) -> tuple:
     """(pages, kv heads, tokens of a page, head width) of a cache in 8 bits."""
-    _check(k_pages, "k_pages", E4M3, (None, num_kv_heads, None, None))
-    NB, KV, bs, D = k_pages.shape
+    try:
+        NB, KV, bs, D = shape = k_pages.shape
+        scales = (NB, KV, bs // BLOCK8)
+        good = (_good(k_pages, E4M3, shape) and _good(v_pages, E4M3, (*scales, D, BLOCK8)) and _good(k_scales, F32, scales)
+                and _good(v_scales, F32, scales) and KV == (num_kv_heads or KV))  # fmt: skip
+    except (AttributeError, ValueError):
+        good = False
+    if not good:
+        _check(k_pages, "k_pages", E4M3, (None, num_kv_heads, None, None))
+        NB, KV, bs, D = k_pages.shape
+        _check(v_pages, "v_pages", E4M3, (NB, KV, bs // BLOCK8, D, BLOCK8))
+        _check(k_scales, "k_scales", F32, (NB, KV, bs // BLOCK8))
+        _check(v_scales, "v_scales", F32, (NB, KV, bs // BLOCK8))
     if bs % BLOCK8 or bs == 0 or D % 64 or not 0 < D <= 256 or NB == 0 or KV == 0:
         raise KernelError(f"a cache in 8 bits has pages of a multiple of {BLOCK8} tokens and heads of 64, 128, 192 or 256, not {bs} and {D}")
-    _check(v_pages, "v_pages", E4M3, (NB, KV, bs // BLOCK8, D, BLOCK8))
-    _check(k_scales, "k_scales", F32, (NB, KV, bs // BLOCK8))
-    _check(v_scales, "v_scales", F32, (NB, KV, bs // BLOCK8))
     return NB, KV, bs, D
+
+
+def _addresses(*tensors) -> list:
+    """`_ptr` of each."""
+    if watch.held is not None:
+        return [_ptr(t) for t in tensors]
+    return [0 if t is None else t.data_ptr() for t in tensors]
+
+
+def _good_or_check(t, name, dtype, shape) -> None:
+    """`_check` of one dtype and a shape without gaps."""
+    if not isinstance(t, torch.Tensor) or not _good(t, dtype, shape):
+        _check(t, name, dtype, shape)
 
 
 def qk_norm_rope_store8(qkv, q_weight, k_weight, cos_sin, slots, q_out, k_pages, v_pages, k_scales, v_scales, num_heads, num_kv_heads, eps,
@@ -830,29 +859,30 @@ def qk_norm_rope_store8(qkv, q_weight, k_weight, cos_sin, slots, q_out, k_pages,
     tokens do: two runs of one call in one block, or one place twice, leave that block undefined.  What is not finite is stored as zero."""
     _check(qkv, "qkv", BF16, (None, num_heads + 2 * num_kv_heads, None))
     T, _, D = qkv.shape
-    _check(q_out, "q_out", BF16, (T, num_heads, D))
+    _good_or_check(q_out, "q_out", BF16, (T, num_heads, D))
     R = 0
     if cos_sin is not None:
         _check(cos_sin, "cos_sin", F32, (T, None, 2))
         R = 2 * cos_sin.shape[1]
     if R > D or R % 8 or D % 64 or not 0 < D <= 256:
         raise KernelError(f"appending in 8 bits: unsupported head width {D} (64, 128, 192 or 256) or rotary width {R} (a multiple of 8)")
-    if (q_weight is None) != (k_weight is None):
-        raise KernelError("q and k norm weights come together")
     w_dtype = BF16
-    if q_weight is not None:
+    if q_weight is not None and k_weight is not None:
         _check(q_weight, "q_weight", (F32, BF16), (D,))
-        _check(k_weight, "k_weight", q_weight.dtype, (D,))
         w_dtype = q_weight.dtype
-    NB, bs = 1, BLOCK8
+        _good_or_check(k_weight, "k_weight", w_dtype, (D,))
+    elif q_weight is not None or k_weight is not None:
+        raise KernelError("q and k norm weights come together")
+    NB, bs, cache = 1, BLOCK8, (None,) * 5
     if store_kv:
-        _check(slots, "slots", I32, (T,))
-        NB, _, bs, width = _check_pages8(k_pages, v_pages, k_scales, v_scales, num_kv_heads)
+        _good_or_check(slots, "slots", I32, (T,))
+        NB, _, bs, width = _pages8(k_pages, v_pages, k_scales, v_scales, num_kv_heads)
         if width != D:
             raise KernelError(f"k_pages has heads of {width}, qkv of {D}")
-    held = (_ptr(slots), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales)) if store_kv else (0,) * 5
-    call("as_qk_norm_rope_store8", _ptr(qkv), _ptr(q_weight), _ptr(k_weight), _DT[w_dtype], _ptr(cos_sin) if R else 0, held[0], _ptr(q_out),
-         *held[1:], NB, T, num_heads, num_kv_heads, D, R, float(eps), bs, int(bool(store_kv)), _stream())  # fmt: skip
+        cache = slots, k_pages, v_pages, k_scales, v_scales
+    p_qkv, p_qw, p_kw, p_cs, p_q, p_slots, *pages = _addresses(qkv, q_weight, k_weight, cos_sin if R else None, q_out, *cache)
+    call("as_qk_norm_rope_store8", p_qkv, p_qw, p_kw, _DT[w_dtype], p_cs, p_slots, p_q, *pages, NB, T, num_heads, num_kv_heads, D, R, float(eps), bs,
+         int(bool(store_kv)), _stream())  # fmt: skip
 
 
 def _up64(n: int) -> int:
@@ -870,12 +900,13 @@ SINGLE8_PARTITIONS = (128, 256, 512, 1024, 2048, 4096, 8192)
 
 
 @functools.lru_cache(maxsize=1024)
-def _partition8(N: int, H: int, KV: int, D: int, span: int, units: int) -> int:
-    """Keys of a partition for N single queries that see up to `span` keys (a multiple of 64)."""
+def _partition8(N: int, H: int, KV: int, D: int, span: int, units: int, capped: bool) -> int:
+    """Keys of a partition for N single queries that see up to `span` keys (a multiple of 64).  Capped scores take a workgroup 1.4 times as long."""
     groups = N * KV
     if groups >= units * 3 // 2:
         return span
     start, key, per_unit = SINGLE8_COSTS[D]
+    key *= 1.4 if capped else 1.0
     memory = groups * span * 2 * D / 7.3e6 + start
 
     def cost(part: int) -> float:
@@ -887,11 +918,11 @@ def _partition8(N: int, H: int, KV: int, D: int, span: int, units: int) -> int:
     return min((span, *(part for part in SINGLE8_PARTITIONS if part < span)), key=cost)
 
 
-def _partitions8(N, H, KV, D, max_context, window, part_size, device, keep_first=0):
+def _partitions8(N, H, KV, D, max_context, window, part_size, device, keep_first=0, capped=False):
     """`_partitions` for the kernel of single queries over 8 bits, whose steps are 64 keys."""
     span = _up64(max_context) if window <= 0 else min(_up64(max_context), _up64(window + STEP8 - 1) + _up64(keep_first))
     if part_size is None:
-        part_size = _partition8(N, H, KV, D, span, compute_units())
+        part_size = _partition8(N, H, KV, D, span, compute_units(), capped)
     if part_size <= 0 or part_size % STEP8:
         raise KernelError(f"attention over 8 bits: partitions are multiples of {STEP8} keys")
     P = max(1, math.ceil(span / part_size))
@@ -900,6 +931,7 @@ def _partitions8(N, H, KV, D, max_context, window, part_size, device, keep_first
     return part_size, P, torch.empty(N * H * P * (D + 2), dtype=F32, device=device)
 
 
+@functools.lru_cache(maxsize=64)
 def _share8(group: int) -> int:
     """Into how many equal groups of at most 16 the query heads of a kv head are cut."""
     return next(n for n in range(1, group + 1) if group % n == 0 and group // n <= 16)
@@ -911,28 +943,31 @@ def attn_single_query8(q, k_pages, v_pages, k_scales, v_scales, items, positions
     _check(q, "q", BF16, (None, None, None))
     T, H, D = q.shape
     sight = _sight(window, keep_first, chunk, softcap, sink, q, out)
-    NB, KV, bs, width = _check_pages8(k_pages, v_pages, k_scales, v_scales)
+    NB, KV, bs, width = _pages8(k_pages, v_pages, k_scales, v_scales)
+    N = T
     if items is not None:
         _check(items, "items", I32, (None,))
-    _check(positions, "positions", I32, (T,))
+        N = items.shape[0]
+    _good_or_check(positions, "positions", I32, (T,))
     if tok_row is not None:
-        _check(tok_row, "tok_row", I32, (T,))
+        _good_or_check(tok_row, "tok_row", I32, (T,))
     _check(block_tables, "block_tables", I32, (None, None))
-    if tok_row is None and block_tables.shape[0] < T:
+    rows, table_width = block_tables.shape
+    if tok_row is None and rows < T:
         raise KernelError(f"attention: {T} tokens that are their own rows need as many block tables")
-    N = T if items is None else items.shape[0]
     if N == 0:
         return
     if H % KV or width != D:
         raise KernelError(f"attention over 8 bits: heads {H}/{KV} of {D} do not fit pages of heads of {width}")
     if not scale > 0:
         raise KernelError("attention over 8 bits: scores have a positive scale")
-    if max_context > block_tables.shape[1] * bs:
+    if max_context > table_width * bs:
         raise KernelError("attention: block tables are shorter than the longest context")
     share = _share8(H // KV)
-    part_size, P, parts = _partitions8(N, H, KV * share, D, max_context, window or chunk, part_size, q.device, sight[1])
-    call("as_attn_single_query8", _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales), NB, _ptr(items), N, _ptr(positions),
-         _ptr(tok_row), _ptr(block_tables), block_tables.shape[1], _ptr(out), _ptr(parts), H, KV * share, D, bs,
+    part_size, P, parts = _partitions8(N, H, KV * share, D, max_context, window or chunk, part_size, q.device, sight[1], softcap > 0)
+    p_q, p_k, p_v, p_ks, p_vs, p_items, p_pos, p_row, p_tables, p_out, p_parts = _addresses(
+        q, k_pages, v_pages, k_scales, v_scales, items, positions, tok_row, block_tables, out, parts)
+    call("as_attn_single_query8", p_q, p_k, p_v, p_ks, p_vs, NB, p_items, N, p_pos, p_row, p_tables, table_width, p_out, p_parts, H, KV * share, D, bs,
          float(scale), *sight, part_size, P, share, _stream())  # fmt: skip
 
 
@@ -985,25 +1020,26 @@ def attn_prefill8(q, k_pages, v_pages, k_scales, v_scales, tiles, block_tables, 
     _check(q, "q", BF16, (None, None, None))
     T, H, D = q.shape
     sight = _sight(window, keep_first, chunk, softcap, sink, q, out)
-    NB, KV, bs, width = _check_pages8(k_pages, v_pages, k_scales, v_scales)
+    NB, KV, bs, width = _pages8(k_pages, v_pages, k_scales, v_scales)
     _check(tiles, "tiles", I32, (None, 4))
     _check(block_tables, "block_tables", I32, (None, None))
-    if tiles.shape[0] == 0:
+    num_tiles, table_width = tiles.shape[0], block_tables.shape[1]
+    if num_tiles == 0:
         return
     if H % KV or width != D:
         raise KernelError(f"prefill attention over 8 bits: heads {H}/{KV} of {D} do not fit pages of heads of {width}")
     if not scale > 0:
         raise KernelError("attention over 8 bits: scores have a positive scale")
-    if max_context > block_tables.shape[1] * bs:
+    if max_context > table_width * bs:
         raise KernelError("attention: block tables are shorter than the longest context")
-    query_tiles, pieces, piece_rounds = _prefill8_plan(tiles.shape[0], H, KV, D, max_context, window or chunk, query_tiles or PREFILL_QUERY_TILES,
+    query_tiles, pieces, piece_rounds = _prefill8_plan(num_tiles, H, KV, D, max_context, window or chunk, query_tiles or PREFILL_QUERY_TILES,
                                                        tile_keys, PREFILL_PIECES, compute_units(), sight[1])  # fmt: skip
     parts = None  # outputs, maxima and sums of the pieces, and how many pieces each item has
     if pieces > 1:
-        parts = torch.empty(T * H * pieces * (D + 2) + tiles.shape[0] * KV * _prefill_units(query_tiles, H // KV), dtype=F32, device=q.device)
-    call("as_attn_prefill8", _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(k_scales), _ptr(v_scales), NB, _ptr(tiles), tiles.shape[0],
-         _ptr(block_tables), block_tables.shape[1], _ptr(out), H, KV, D, bs, float(scale), *sight, int(query_tiles), pieces, piece_rounds, _ptr(parts), T,
-         _stream())  # fmt: skip
+        parts = torch.empty(T * H * pieces * (D + 2) + num_tiles * KV * _prefill_units(query_tiles, H // KV), dtype=F32, device=q.device)
+    p_q, p_k, p_v, p_ks, p_vs, p_tiles, p_tables, p_out, p_parts = _addresses(q, k_pages, v_pages, k_scales, v_scales, tiles, block_tables, out, parts)
+    call("as_attn_prefill8", p_q, p_k, p_v, p_ks, p_vs, NB, p_tiles, num_tiles, p_tables, table_width, p_out, H, KV, D, bs, float(scale), *sight,
+         int(query_tiles), pieces, piece_rounds, p_parts, T, _stream())  # fmt: skip
 
 
 SKINNY_MAX_ROWS = 16  # up to here the bf16 product streams the weights through our own kernel
