@@ -44,13 +44,14 @@ def slot_of(block_table: list, position: int, block_size: int) -> int:
 
 
 class PagedLayerView:
-    """What an attention mixer sees of its cache in one step."""
+    """What an attention mixer sees of its cache in one step; k_scales, v_scales: of a cache in 8 bits, else None."""
 
-    __slots__ = ("k_pages", "v_pages", "slots", "block_tables", "writes", "block_size")
+    __slots__ = ("k_pages", "v_pages", "slots", "block_tables", "writes", "block_size", "k_scales", "v_scales")
 
-    def __init__(self, k_pages, v_pages, slots, block_tables, writes, block_size):
+    def __init__(self, k_pages, v_pages, slots, block_tables, writes, block_size, k_scales=None, v_scales=None):
         self.k_pages, self.v_pages, self.slots, self.block_tables = k_pages, v_pages, slots, block_tables
         self.writes, self.block_size = writes, block_size
+        self.k_scales, self.v_scales = k_scales, v_scales
 
 
 class StateLayerView:
@@ -364,7 +365,8 @@ class StepBatch:
         kind, gi, _ = found
         if kind == "paged":
             _, k_pages, v_pages = self.pools.pages(cache_id)
-            return PagedLayerView(k_pages, v_pages, self.group_slots[gi], self.group_tables[gi], writes, self.block_size)
+            return PagedLayerView(k_pages, v_pages, self.group_slots[gi], self.group_tables[gi], writes, self.block_size,
+                                  *self.pools.scales_of(cache_id))  # fmt: skip
         _, state = self.pools.state_of(cache_id)
         return StateLayerView(state, self.row_slots, writes)
 

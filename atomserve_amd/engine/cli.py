@@ -79,6 +79,9 @@ def build_parser() -> argparse.ArgumentParser:
                    help="GiB of memory for the KV cache, or 'auto' for all that the weights leave free; "
                         "reduced with a note if the GPU has less left")  # fmt: skip
     p.add_argument("--block-size", type=int, default=16, help="tokens per KV block")
+    p.add_argument("--cache-bits", type=int, choices=(0, 8), default=0,
+                   help="8: keys and values as 8-bit numbers (e4m3) with a scale for every 16 tokens and head, twice the tokens in "
+                        "the same memory (bf16, heads of 64 to 256, blocks of a multiple of 16 tokens); 0: as the weights")  # fmt: skip
     p.add_argument("--max-num-seqs", type=int, default=32, help="most requests running at once")
     p.add_argument("--max-batched-tokens", type=int, default=512,
                    help="token budget of one forward pass; smaller bounds the stall a long prompt causes "
@@ -173,6 +176,9 @@ def main(argv=None) -> int:
         print(f"atomserve: no config.json at {config_path}", file=sys.stderr)
         return 1
     dtype = torch.bfloat16 if args.dtype == "bf16" else torch.float32
+    if args.cache_bits == 8 and args.block_size % 16:
+        print(f"atomserve: a cache in 8 bits has blocks of a multiple of 16 tokens, not {args.block_size}", file=sys.stderr)
+        return 1
     try:  # what is wrong with the folder is a message, not a traceback
         with open(config_path) as f:
             raw = json.load(f)
@@ -183,7 +189,8 @@ def main(argv=None) -> int:
 
             config = arch.complete(config, checkpoint_shapes_of(model_dir))
         print(f"Loading {args.model} ({args.dtype}, {arch.name}) ...", file=sys.stderr, flush=True)
-        model = DecoderModel(arch.build_plan(config), dtype, "cuda:0", stream_copies=not args.no_stream_copies)
+        model = DecoderModel(arch.build_plan(config), dtype, "cuda:0", stream_copies=not args.no_stream_copies,
+                             cache_bits=args.cache_bits)  # fmt: skip
         if args.random_weights is not None:
             source = DictSource(random_checkpoint(arch, config, args.random_weights, dtype=dtype, device="cuda:0"))
             bind_checkpoint(model, arch, config, source, where="(random)")

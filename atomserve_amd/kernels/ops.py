@@ -931,6 +931,12 @@ def _partitions8(N, H, KV, D, max_context, window, part_size, device, keep_first
     return part_size, P, torch.empty(N * H * P * (D + 2), dtype=F32, device=device)
 
 
+def contexts_cut8(rows: int, H: int, KV: int, D: int, context: int, window: int = 0, keep_first: int = 0) -> bool:
+    """`contexts_cut` for `attn_single_query8`."""
+    share = _share8(H // KV)
+    return _partitions8(rows, H, KV * share, D, context, window, None, "meta", keep_first)[1] > 1
+
+
 @functools.lru_cache(maxsize=64)
 def _share8(group: int) -> int:
     """Into how many equal groups of at most 16 the query heads of a kv head are cut."""

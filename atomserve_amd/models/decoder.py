@@ -15,14 +15,18 @@ from atomserve_amd.parts.plan import ModelPlan
 
 
 class DecoderModel:
-    def __init__(self, plan: ModelPlan, dtype: torch.dtype, device, stream_copies: bool = True):
+    def __init__(self, plan: ModelPlan, dtype: torch.dtype, device, stream_copies: bool = True, cache_bits: int = 0):
         """stream_copies: keep the matrices that decode steps stream a second time, in the order their
-        kernels read them (`ops.Streamed`): faster decode steps for the weights' bytes again."""
+        kernels read them (`ops.Streamed`): faster decode steps for the weights' bytes again.
+        cache_bits: 8 for keys and values in 8 bits in every layer whose mixer reads such a cache (twice the tokens in the
+        same memory); ValueError where a layer of that kind has heads that it does not take, or the model has none."""
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"compute dtype must be float32 or bfloat16, got {dtype}")
+        if cache_bits not in (0, 8):
+            raise ValueError(f"a cache holds the compute dtype (0) or 8 bits, not {cache_bits}")
         self.plan = plan
         self.env = BuildEnv(dtype=dtype, device=torch.device(device), stream_copies=bool(stream_copies),
-                            products=ops.ProductChoices())  # fmt: skip
+                            cache_bits=cache_bits, products=ops.ProductChoices())  # fmt: skip
         self.blocks = [build("arrangement", spec, self.env) for spec in plan.layers]
         self.final_norm = build("norm", plan.final_norm, self.env)
         self.embed_norm = build("norm", plan.embed_norm, self.env) if plan.embed_norm is not None else None
@@ -35,6 +39,8 @@ class DecoderModel:
                 raise ValueError(f"run list names layer {r.layer}, the plan has {len(self.blocks)}")
         self.embed_weight = None
         self.head_weight = None
+        if cache_bits and not any(getattr(req, "bits", 0) for req in self.cache_requests().values()):
+            raise ValueError("no layer of this model keeps its keys and values in 8 bits")
         self.stretches = repeats.stretches(plan, self.blocks)  # which layers are like the ones before them
 
     @property
@@ -138,8 +144,10 @@ class DecoderModel:
 
     def contexts_cut(self, rows: int, context: int, block_size: int) -> bool:
         """Whether a decode step of `rows` rows and contexts of up to `context` tokens cuts some layer's contexts into partitions."""
-        return any(ops.contexts_cut(rows, H, KV, D, self.env.dtype, block_size, context, window, keep)
-                   for H, KV, D, window, keep in {q for block in self.blocks for q in block.parts()["mixer"].single_queries()})  # fmt: skip
+        mixers = [block.parts()["mixer"] for block in self.blocks]
+        return any(ops.contexts_cut8(rows, H, KV, D, context, window, keep) if bits else
+                   ops.contexts_cut(rows, H, KV, D, self.env.dtype, block_size, context, window, keep)
+                   for bits, (H, KV, D, window, keep) in {(getattr(mixer, "cache_bits", 0), q) for mixer in mixers for q in mixer.single_queries()})  # fmt: skip
 
     def forward(self, step, logits: torch.Tensor = None) -> torch.Tensor:
         """Run this step's tokens through every run of the plan; returns fp32 logits

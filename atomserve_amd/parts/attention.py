@@ -53,6 +53,11 @@ class Attention(Mixer):
                 f"(a position part that declares pairs = 'half'); {s.position.kind!r} declares "
                 f"{getattr(self.position, 'pairs', None)!r}"
             )
+        rotary = getattr(s.position, "rotary_dim", 0) if s.position is not None else 0
+        if env.cache_bits == 8 and not ops.cache8_supported(env.dtype, s.num_heads, s.num_kv_heads, s.head_dim, ops.BLOCK8, rotary):
+            raise ValueError(f"a cache in 8 bits takes bfloat16 heads of 64, 128, 192 or 256 that turn in a multiple of 8 coordinates, not "
+                             f"{env.dtype} heads of {s.head_dim} that turn in {rotary}")  # fmt: skip
+        self.cache_bits = env.cache_bits
         self.q_norm_weight = self.k_norm_weight = None
 
     def repeats(self, step) -> bool:
@@ -81,7 +86,7 @@ class Attention(Mixer):
 
     def cache_request(self):
         s = self.spec
-        return PagedCacheRequest(s.num_kv_heads, s.head_dim, s.window)
+        return PagedCacheRequest(s.num_kv_heads, s.head_dim, s.window, bits=self.cache_bits)
 
     def row_split(self):
         return (SHORT_ROW, TILE_Q)
@@ -107,8 +112,11 @@ class Attention(Mixer):
         eps = s.qk_norm.eps if s.qk_norm is not None else 0.0
         rotary = 2 * cos_sin.shape[1] if cos_sin is not None else 0
         case = env.dtype, H, KV, D, cache.block_size, rotary, s.qk_norm is not None
+        eight = getattr(cache, "k_scales", None) is not None
         fresh = None  # a decode step: norm, rotation, the cache store and attention in one kernel
-        if step.decode_only and ops.attn_decode_fresh_supported(*case):
+        if eight:
+            pass
+        elif step.decode_only and ops.attn_decode_fresh_supported(*case):
             fresh = ops.attn_decode_fresh
         elif step.decode_only and ops.attn_f32_fresh_supported(*case) and not (self.q_norm_weight.data_ptr() | self.k_norm_weight.data_ptr()) & 15:
             fresh = ops.attn_f32_fresh
@@ -121,10 +129,11 @@ class Attention(Mixer):
             )  # fmt: skip
         else:
             q = torch.empty((T, H, D), dtype=env.dtype, device=device)
-            ops.qk_norm_rope_store(
-                qkv.view(T, H + 2 * KV, D), self.q_norm_weight, self.k_norm_weight, cos_sin, cache.slots, q,
-                cache.k_pages, cache.v_pages, H, KV, eps, store_kv=cache.writes,
-            )  # fmt: skip
+            heads = qkv.view(T, H + 2 * KV, D), self.q_norm_weight, self.k_norm_weight, cos_sin, cache.slots, q, cache.k_pages, cache.v_pages
+            if eight:
+                ops.qk_norm_rope_store8(*heads, cache.k_scales, cache.v_scales, H, KV, eps, store_kv=cache.writes)
+            else:
+                ops.qk_norm_rope_store(*heads, H, KV, eps, store_kv=cache.writes)
             out = torch.empty((T, H, D), dtype=env.dtype, device=device)
             self.attend(q, out, step, cache)
         if residual is not None and next_norm is not None:
@@ -140,7 +149,22 @@ class Attention(Mixer):
         return y
 
     def attend(self, q, out, step, cache) -> None:
-        attend(q, out, step, cache, self.spec.scale, self.spec.window, self.row_split())
+        over = attend8 if getattr(cache, "k_scales", None) is not None else attend
+        over(q, out, step, cache, self.spec.scale, self.spec.window, self.row_split())
+
+
+def attend8(q, out, step, cache, scale: float, window: int, split) -> None:
+    """`attend` over a cache in 8 bits: single tokens and short rows as single queries, long rows in tiles."""
+    pages = cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales
+    if step.decode_only:  # token t is row t
+        ops.attn_single_query8(q, *pages, step.all_tokens, step.positions, None, cache.block_tables, out, scale, window, step.max_context)
+        return
+    rows = step.split(split)
+    if rows.num_short_tokens:
+        ops.attn_single_query8(q, *pages, rows.short_tokens, step.positions, step.tok_row, cache.block_tables, out, scale, window,
+                               rows.max_short_context)  # fmt: skip
+    if rows.num_long_tiles:
+        ops.attn_prefill8(q, *pages, rows.long_tiles, cache.block_tables, out, scale, window, rows.max_tile_context, tile_keys=rows.tile_keys)
 
 
 def attend(q, out, step, cache, scale: float, window: int, split, wide: bool = False, **sight) -> None:

@@ -49,6 +49,7 @@ class PagedCacheRequest:
     head_dim: int
     window: int = 0  # 0: all keys are kept; > 0: pages wholly behind the window are given back
     keep_first: int = 0  # with a window: the sequence's first tokens that stay visible; their pages are never given back
+    bits: int = 0  # 8: e4m3 numbers under a scale for 16 tokens and head (`ops.qk_norm_rope_store8`); 0: the compute dtype
 
 
 @dataclass(frozen=True)
@@ -102,6 +103,8 @@ class BuildEnv:
     # whether matrices that decode steps stream are kept a second time in the order their kernels read
     # them (faster steps for the weights' bytes again); a part asks `ops.Streamed(w, env.stream_copies)`
     stream_copies: bool = True
+    # 8: mixers whose kernels read a cache in 8 bits ask for one (`PagedCacheRequest.bits`); 0: the compute dtype everywhere
+    cache_bits: int = 0
     # which of the library's kernels the model's matrix products run (`ops.ProductChoices`): the model's own
     # object, which its parts hand to `ops.gemm`; None: the one the process shares
     products: Any = None
@@ -193,6 +196,7 @@ class Mixer(Part):
     #   `takes_split_sums` it may return its output as `SplitSums`.
     takes_pending_norm = False
     adds_to_residual = False
+    cache_bits = 0  # 8 where its single queries read a cache in 8 bits
 
     def cache_request(self) -> Optional[Any]:
         """What this mixer keeps between steps: a `PagedCacheRequest`, a `StateCacheRequest`, None, or a

@@ -68,6 +68,7 @@ def parse_args():
     p.add_argument("--dtype", choices=["bf16", "fp32"], default="bf16")
     p.add_argument("--points", default="1,64", help="other decode batch sizes to measure (fewer steps each)")
     p.add_argument("--block-size", type=int, default=16, help="tokens per cache page")
+    p.add_argument("--cache-bits", type=int, choices=(0, 8), default=0, help="8: keys and values in 8 bits (bf16 only); 0: as the weights")
     p.add_argument("--no-prefill", action="store_true")
     p.add_argument("--prefill-tokens", type=int, default=2048, help="length of the prompt whose prefill is timed "
                    "(longer than the step budget: in portions of it)")  # fmt: skip
@@ -165,6 +166,7 @@ def mixed_workload(args, model, config, full_layers: int) -> dict:
             "seq_len": longest, "decoded_each": decoded, "chunk_budget": budget, "block_size": block,
             "shared_prefix": 32, "parallelism": "single GPU",
             "sampling": "greedy" if args.greedy else "temperature 0.6 top-k 20 top-p 0.95",
+            **({"cache_bits": args.cache_bits} if args.cache_bits else {}),
         },
         "run_ms": round(dt * 1e3, 1),
         "prompt_tokens": prompt_tokens,
@@ -452,6 +454,7 @@ def main() -> int:
     from atomserve_amd.config.registry import architecture_for
     from atomserve_amd.engine.engine import create_engine
     from atomserve_amd.engine.sequence import SamplingParams
+    from atomserve_amd.cache.pools import CachePools
     from atomserve_amd.models.decoder import DecoderModel
     from atomserve_amd.weights.loader import DictSource, bind_checkpoint
     from atomserve_amd.weights.random_init import random_checkpoint
@@ -465,7 +468,7 @@ def main() -> int:
     full_layers = SIZES[args.sizes]["num_layers"]
     config = Qwen3Config(**{**SIZES[args.sizes], "num_layers": args.layers or full_layers})
     arch = architecture_for(config.to_dict())
-    model = DecoderModel(arch.build_plan(config), dtype, device)
+    model = DecoderModel(arch.build_plan(config), dtype, device, cache_bits=args.cache_bits)
     bind_checkpoint(model, arch, config, DictSource(random_checkpoint(arch, config, seed=0, dtype=dtype, device=device)))
     torch.cuda.synchronize()
     if args.workload == "mixed":
@@ -490,7 +493,7 @@ def main() -> int:
     layer_params = c.hidden_size * (c.num_heads + 2 * c.num_kv_heads) * c.head_dim + c.num_heads * c.head_dim * c.hidden_size \
         + 3 * c.hidden_size * c.intermediate_size  # fmt: skip
     weight_bytes = (layer_params * c.num_layers + c.vocab_size * c.hidden_size) * itemsize
-    kv_bytes_per_token = c.num_layers * 2 * c.num_kv_heads * c.head_dim * itemsize
+    kv_bytes_per_token = CachePools.bytes_per_block(model.cache_requests(), block, dtype) / block
 
     host_phases = {}
 
@@ -580,6 +583,7 @@ def main() -> int:
             "seq_len": args.context, "shortest_context": args.shortest_context or args.context, "max_context": max_len, "block_size": block,
             "step_budget": engine_config.max_num_batched_tokens, "parallelism": "single GPU",
             "sampling": "greedy" if args.greedy else "temperature 0.6 top-k 20 top-p 0.95",
+            **({"cache_bits": args.cache_bits} if args.cache_bits else {}),
         },
         "roofline": roofline(args.batch, mean_ctx, ms),
         "points": points,

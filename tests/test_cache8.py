@@ -124,3 +124,71 @@ def test_which_heads_the_cache_takes():
     assert not takes(F32, 32, 8, 128, 16) and not takes(BF16, 32, 8, 96, 16) and not takes(BF16, 32, 8, 128, 8) and not takes(BF16, 9, 2, 128, 16)
     assert not takes(BF16, 32, 8, 128, 16, 12) and not takes(BF16, 8, 8, 320, 16)
     assert [ops._share8(g) for g in (1, 7, 16, 17, 24, 32, 40)] == [1, 1, 1, 17, 2, 2, 4]
+
+
+# ---- pools and the models that ask for them -----------------------------------------------------------
+
+
+def real(fn):
+    """Runs with real tensors on the host."""
+    from torch.utils._python_dispatch import _disable_current_modes
+
+    def wrapped(*args, **kw):
+        with _disable_current_modes():
+            return fn(*args, **kw)
+
+    wrapped.__name__ = fn.__name__
+    return wrapped
+
+
+@real
+def test_pools_in_8_bits():
+    from atomserve_amd.cache import CacheManager, CachePools
+    from atomserve_amd.parts.base import PagedCacheRequest
+
+    requests = {0: PagedCacheRequest(2, 64, bits=8), 1: PagedCacheRequest(2, 64), 2: PagedCacheRequest(2, 64, bits=8)}
+    manager = CacheManager(requests, 32, 5, 2)
+    assert [g.cache_ids for g in manager.paged_groups] == [[0, 2], [1]]
+    pools = CachePools(manager, BF16, "cpu")
+    _, k, v = pools.pages(2)
+    ks, vs = pools.scales_of(2)
+    assert k.dtype == v.dtype == E4M3 and k.shape == (5, 2, 32, 64) and v.shape == (5, 2, 2, 64, 16) and k.is_contiguous() and v.is_contiguous()
+    assert ks.shape == vs.shape == (5, 2, 2) and ks.dtype == F32 and not ks.any() and not k.view(torch.uint8).any()
+    _, k, v = pools.pages(1)
+    assert k.dtype == BF16 and v.shape == (5, 2, 64, 32) and pools.scales_of(1) == (None, None)
+    held = sum(t.numel() * t.element_size() for t in [*pools.paged, *(s for s in pools.scales if s is not None)])
+    assert held == 5 * CachePools.bytes_per_block(requests, 32, BF16)
+    for bad, pages in ((PagedCacheRequest(2, 64, bits=8), 24), (PagedCacheRequest(2, 64, bits=4), 16)):
+        with pytest.raises(ValueError):
+            CachePools(CacheManager({0: bad}, pages, 5, 2), BF16, "cpu")
+
+
+@real
+def test_which_models_keep_8_bits():
+    from atomserve_amd.config.registry import architecture_for
+    from atomserve_amd.models.decoder import DecoderModel
+    from tests.conftest import TINY_A
+    from tests.mumizen_cases import CASES
+
+    def model(raw, dtype=BF16, bits=8):
+        arch = architecture_for(raw)
+        return DecoderModel(arch.build_plan(arch.parse_config(raw)), dtype, "cpu", cache_bits=bits)
+
+    wide = {**TINY_A, "head_dim": 64}
+    assert {r.bits for r in model(wide).cache_requests().values()} == {8}
+    assert {r.bits for r in model(wide, bits=0).cache_requests().values()} == {0}
+    for raw, dtype in ((TINY_A, BF16), (wide, F32)):  # heads of 16; 32-bit heads
+        with pytest.raises(ValueError, match="bfloat16 heads of 64"):
+            model(raw, dtype)
+    with pytest.raises(ValueError, match="no layer"):
+        model(CASES["latent_first"])
+    with pytest.raises(ValueError, match="8 bits, not 4"):
+        model(wide, bits=4)
+
+
+def test_the_command_line_names_the_cache():
+    from atomserve_amd.engine.cli import build_parser
+
+    assert build_parser().parse_args(["m"]).cache_bits == 0 and build_parser().parse_args(["m", "--cache-bits", "8"]).cache_bits == 8
+    with pytest.raises(SystemExit):
+        build_parser().parse_args(["m", "--cache-bits", "4"])
