@@ -91,6 +91,7 @@ SIGNATURES = {
     "as_attn_f32_fresh": ("attention", [P, P, P, P, P, F, I, P, P, P, I, P, P, I, P, P, P, P, I, I, I, I, F, I, I, I, P]),
     "as_qk_norm_rope_store8": ("cache8", [P, P, P, I, P, P, P, P, P, P, P, I, I, I, I, I, I, F, I, I, P]),
     "as_attn_single_query8": ("cache8", [P, P, P, P, P, I, P, I, P, P, P, I, P, P, I, I, I, I, F, I, I, I, F, I, P, I, I, I, I, P]),
+    "as_attn_decode_fresh8": ("cache8", [P, P, P, I, P, P, F, I, P, P, P, P, I, P, I, P, P, I, P, P, I, I, I, I, I, F, I, I, I, P]),
     "as_attn_prefill8": ("cache8", [P, P, P, P, P, I, P, I, P, I, P, I, I, I, I, F, I, I, I, F, I, P, I, I, I, I, P, I, P]),
     "as_gemm_f32": ("gemm_f32", [P, P, P, I, I, I, I, P]),
     "as_gemm_f32_gated": ("gemm_f32", [P, P, P, I, I, I, I, P]),

@@ -977,6 +977,60 @@ def attn_single_query8(q, k_pages, v_pages, k_scales, v_scales, items, positions
          float(scale), *sight, part_size, P, share, _stream())  # fmt: skip
 
 
+def attn_decode_fresh8_supported(dtype, num_heads: int, num_kv_heads: int, head_dim: int, block_size: int, rotary_dim: int) -> bool:
+    """Whether `attn_decode_fresh8` takes this case: what `cache8_supported` names, at most 16 query heads to a kv head."""
+    return cache8_supported(dtype, num_heads, num_kv_heads, head_dim, block_size, rotary_dim) and num_heads // num_kv_heads <= 16
+
+
+def attn_decode_fresh8(qkv, q_weight, k_weight, cos_sin, slots, eps, store_kv, k_pages, v_pages, k_scales, v_scales, positions, block_tables, out,
+                       num_heads, scale, window, max_context, part_size=None, order=None) -> None:  # fmt: skip
+    """`attn_decode_fresh` over a cache in 8 bits: what `qk_norm_rope_store8` and then `attn_single_query8` do for tokens that are their own rows (token t
+    reads block table t), in one kernel and with the same numbers; the per-head norm and the rotation may be missing.  slots[t] is the place that block
+    table t names for positions[t], or negative: the token is attended and not kept."""
+    _check(qkv, "qkv", BF16, (None, None, None))
+    T, heads, D = qkv.shape
+    H = num_heads
+    NB, KV, bs, width = _pages8(k_pages, v_pages, k_scales, v_scales)
+    R = 0
+    if cos_sin is not None:
+        _check(cos_sin, "cos_sin", F32, (T, None, 2))
+        R = 2 * cos_sin.shape[1]
+    if heads != H + 2 * KV or width != D or R > D or not attn_decode_fresh8_supported(BF16, H, KV, D, bs, R):
+        raise KernelError(f"attention from fresh projections over 8 bits: unsupported heads {H}/{KV} of {heads} in qkv, head width {D} ({width} in the "
+                          f"pages) or rotary width {R}")  # fmt: skip
+    _good_or_check(out, "out", BF16, (T, H, D))
+    _good_or_check(positions, "positions", I32, (T,))
+    _check(block_tables, "block_tables", I32, (None, None))
+    rows, table_width = block_tables.shape
+    if rows < T:
+        raise KernelError(f"attention: {T} tokens that are their own rows need as many block tables")
+    w_dtype = BF16
+    if q_weight is not None and k_weight is not None:
+        _check(q_weight, "q_weight", (F32, BF16), (D,))
+        w_dtype = q_weight.dtype
+        _good_or_check(k_weight, "k_weight", w_dtype, (D,))
+    elif q_weight is not None or k_weight is not None:
+        raise KernelError("q and k norm weights come together")
+    if store_kv:
+        _good_or_check(slots, "slots", I32, (T,))
+    if order is not None:
+        _good_or_check(order, "order", I32, (T,))
+    if window < 0:
+        raise KernelError("attention: a window is not negative")
+    if T == 0:
+        return
+    if not scale > 0:
+        raise KernelError("attention over 8 bits: scores have a positive scale")
+    if max_context > table_width * bs:
+        raise KernelError("attention: block tables are shorter than the longest context")
+    part_size, P, parts = _partitions8(T, H, KV, D, max_context, window, part_size, qkv.device)
+    p_qkv, p_qw, p_kw, p_cs, p_slots, p_k, p_v, p_ks, p_vs, p_order, p_pos, p_tables, p_out, p_parts = _addresses(
+        qkv, q_weight, k_weight, cos_sin if R else None, slots if store_kv else None, k_pages, v_pages, k_scales, v_scales, order, positions,
+        block_tables, out, parts)  # fmt: skip
+    call("as_attn_decode_fresh8", p_qkv, p_qw, p_kw, _DT[w_dtype], p_cs, p_slots, float(eps), int(bool(store_kv)), p_k, p_v, p_ks, p_vs, NB, p_order, T,
+         p_pos, p_tables, table_width, p_out, p_parts, H, KV, D, R, bs, float(scale), int(window), part_size, P, _stream())  # fmt: skip
+
+
 # What a step of portions over 8 bits costs, in microseconds fitted to the kernel's times of 435 steps (1 to 16 portions of 9 to 2,048 tokens behind 0 to
 # 30,000; 16 to 64 heads of 64, 128, 192 and 256; 256 compute units), by (column tiles of 16 queries that a wave owns, head width): a round of 64 keys where a
 # workgroup has a compute unit to itself, a round where all places are taken, and the places.  Workgroups are counted as far as items are long enough to be

@@ -115,7 +115,8 @@ class Attention(Mixer):
         eight = getattr(cache, "k_scales", None) is not None
         fresh = None  # a decode step: norm, rotation, the cache store and attention in one kernel
         if eight:
-            pass
+            if step.decode_only and ops.attn_decode_fresh8_supported(env.dtype, H, KV, D, cache.block_size, rotary):
+                fresh = ops.attn_decode_fresh8
         elif step.decode_only and ops.attn_decode_fresh_supported(*case):
             fresh = ops.attn_decode_fresh
         elif step.decode_only and ops.attn_f32_fresh_supported(*case) and not (self.q_norm_weight.data_ptr() | self.k_norm_weight.data_ptr()) & 15:
@@ -124,8 +125,8 @@ class Attention(Mixer):
             out = torch.empty((T, H, D), dtype=env.dtype, device=device)
             fresh(
                 qkv.view(T, H + 2 * KV, D), self.q_norm_weight, self.k_norm_weight, cos_sin, cache.slots, eps,
-                cache.writes, cache.k_pages, cache.v_pages, step.positions, cache.block_tables, out, H, s.scale,
-                s.window, step.max_context, order=step.all_tokens,
+                cache.writes, cache.k_pages, cache.v_pages, *((cache.k_scales, cache.v_scales) if eight else ()),
+                step.positions, cache.block_tables, out, H, s.scale, s.window, step.max_context, order=step.all_tokens,
             )  # fmt: skip
         else:
             q = torch.empty((T, H, D), dtype=env.dtype, device=device)

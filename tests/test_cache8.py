@@ -50,13 +50,20 @@ def prompt(T=70, H=4, KV=2, D=64, **kw):
     ops.attn_prefill8(**{**args, **kw})
 
 
-@pytest.mark.parametrize("call", [append, single, prompt])
+def fresh(T=3, H=4, KV=2, D=64, **kw):
+    args = {"qkv": tensor(T, H + 2 * KV, D), "q_weight": None, "k_weight": None, "cos_sin": tensor(T, D // 2, 2, dtype=F32),
+            "slots": tensor(T, dtype=I32), "eps": 1e-6, "store_kv": True, **cache(KV, D=D), "positions": tensor(T, dtype=I32),
+            "block_tables": tensor(T, 4, dtype=I32), "out": tensor(T, H, D), "num_heads": H, "scale": 0.1, "window": 0, "max_context": 64}  # fmt: skip
+    ops.attn_decode_fresh8(**{**args, **kw})
+
+
+@pytest.mark.parametrize("call", [append, single, prompt, fresh])
 def test_what_fits_goes_to_the_kernel(call):
     with pytest.raises(AssertionError, match="would have been launched"):
         call()
 
 
-@pytest.mark.parametrize("call", [append, single, prompt])
+@pytest.mark.parametrize("call", [append, single, prompt, fresh])
 @pytest.mark.parametrize("wrong", [
     {"k_pages": lambda: tensor(4, 2, 16, 64, dtype=BF16)},  # not 8 bits
     {"v_pages": lambda: tensor(4, 2, 64, 16, dtype=E4M3)},  # the layout of a 16-bit cache
@@ -72,7 +79,7 @@ def test_pages_that_do_not_fit_are_refused(call, wrong):
         call(**{k: v() for k, v in wrong.items()})
 
 
-@pytest.mark.parametrize("call", [append, single, prompt])
+@pytest.mark.parametrize("call", [append, single, prompt, fresh])
 @pytest.mark.parametrize("D,bs", [(32, 16), (96, 16), (320, 16), (64, 24), (64, 8)])
 def test_heads_and_pages_that_no_kernel_takes_are_refused(call, D, bs):
     with pytest.raises(ops.KernelError):
@@ -96,7 +103,7 @@ def test_appending_refuses(wrong):
     {"q": lambda: tensor(3, 4, 128), "out": lambda: tensor(3, 4, 128)}, {"positions": lambda: tensor(2, dtype=I32)},
     {"block_tables": lambda: tensor(2, 4, dtype=I32)}, {"max_context": lambda: 65}, {"window": lambda: -1}, {"softcap": lambda: -1.0},
     {"window": lambda: 5, "chunk": lambda: 5}, {"part_size": lambda: 32}, {"part_size": lambda: 96}, {"part_size": lambda: 0},
-    {"sink": lambda: tensor(3, dtype=F32)}, {"items": lambda: tensor(2, dtype=torch.int64)}, {"tok_row": lambda: tensor(2, dtype=I32)},
+    {"sink": lambda: tensor(3, dtype=F32)}, {"scale": lambda: 0.0}, {"items": lambda: tensor(2, dtype=torch.int64)}, {"tok_row": lambda: tensor(2, dtype=I32)},
 ])  # fmt: skip
 def test_single_queries_refuse(wrong):
     with pytest.raises(ops.KernelError):
@@ -113,9 +120,23 @@ def test_prompts_refuse(wrong):
         prompt(**{k: v() for k, v in wrong.items()})
 
 
+@pytest.mark.parametrize("wrong", [
+    {"qkv": lambda: tensor(3, 8, 64, dtype=F32)}, {"qkv": lambda: tensor(3, 9, 64)}, {"num_heads": lambda: 3}, {"out": lambda: tensor(3, 4, 64, dtype=F32)},
+    {"slots": lambda: tensor(2, dtype=I32)}, {"cos_sin": lambda: tensor(3, 34, 2, dtype=F32)}, {"cos_sin": lambda: tensor(2, 32, 2, dtype=F32)},
+    {"q_weight": lambda: tensor(64)}, {"positions": lambda: tensor(4, dtype=I32)}, {"order": lambda: tensor(2, dtype=I32)},
+    {"block_tables": lambda: tensor(2, 4, dtype=I32)}, {"max_context": lambda: 65}, {"window": lambda: -1}, {"scale": lambda: 0.0},
+    {"scale": lambda: -1.0}, {"part_size": lambda: 32},
+    {"qkv": lambda: tensor(3, 34 + 4, 64), "num_heads": lambda: 34, "out": lambda: tensor(3, 34, 64)},  # 17 heads to a kv head
+])  # fmt: skip
+def test_decode_steps_from_the_projection_refuse(wrong):
+    with pytest.raises(ops.KernelError):
+        fresh(**{k: v() for k, v in wrong.items()})
+
+
 def test_nothing_to_do_launches_nothing():
     single(items=tensor(0, dtype=I32))
     prompt(tiles=tensor(0, 4, dtype=I32))
+    fresh(T=0)
 
 
 def test_which_heads_the_cache_takes():

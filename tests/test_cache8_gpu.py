@@ -365,3 +365,40 @@ def test_one_run_of_them_together(ops):
             check(r, done[r], q[r], out[r])
         done = [n + 1 for n in done]
     a.check([slots(r, p) for r in (0, 1) for p in range(done[r])], 2)
+
+
+@pytest.mark.parametrize("D", [64, 128, 192, 256])
+@pytest.mark.parametrize("H,KV,bs,rotary,norm", [(4, 2, 16, 1.0, F32), (16, 1, 48, 0.5, BF16), (21, 3, 32, 0.0, None)])
+@pytest.mark.parametrize("part,window", [(None, 0), (64, 0), (2048, 0), (128, 70)])
+def test_a_decode_step_from_the_projection_is_append_and_attention(ops, D, H, KV, bs, rotary, norm, part, window):
+    """Bit for bit, results and cache: blocks that are new, go on, or whose scale grows; a token that is not kept; one that the pages hold already; one that sees
+    nothing."""
+    lengths = [1, 2, 16, 17, 33, 64, 65, 100, 300, 0]
+    cache, tables, g = requests(KV, D, bs, lengths)
+    T = len(lengths)
+    for scales in cache[2:]:  # of earlier tokens: some far smaller than what comes, so that blocks are rewritten
+        scales.mul_(torch.exp2(torch.randint(-9, 4, scales.shape, generator=g, device=DEV).float()))
+    qkv = (torch.randn(T, H + 2 * KV, D, generator=g, device=DEV) * torch.exp(torch.randn(T, 1, 1, generator=g, device=DEV))).to(BF16)
+    gains = [None, None] if norm is None else [(1 + 0.3 * torch.randn(D, generator=g, device=DEV)).to(norm) for _ in range(2)]
+    R = int(D * rotary)
+    cos_sin = plain.positions_angles([max(n - 1, 0) for n in lengths], R).to(DEV) if R else None
+    slots = [tables[t][(n - 1) // bs] * bs + (n - 1) % bs if n else -1 for t, n in enumerate(lengths)]
+    slots[4] = -1
+    positions, order, scale = i32([n - 1 for n in lengths]), i32([3, 1, 0, 2, 9, 8, 7, 6, 5, 4]), plain.default_scale(D)
+    for store in (True, False):
+        one, two = [x.clone() for x in cache], [x.clone() for x in cache]
+        out = [torch.full((T, H, D), 7.0, dtype=BF16, device=DEV) for _ in range(2)]
+        ops.attn_decode_fresh8(qkv, *gains, cos_sin, i32(slots), 1e-6, store, *one, positions, i32(tables), out[0], H, scale, window, 300, part_size=part,
+                               order=order)  # fmt: skip
+        q = torch.empty((T, H, D), dtype=BF16, device=DEV)
+        kept = slots if store else [-1] * T
+        ops.qk_norm_rope_store8(qkv, *gains, cos_sin, i32(kept), q, *two, H, KV, 1e-6, store_kv=store)
+        ops.attn_single_query8(q, *two, order, positions, None, i32(tables), out[1], scale, window, 300, part_size=part)
+        same = [t for t in range(T) if t != 4 or not store]  # token 4 attends itself, which two kernels cannot
+        assert torch.equal(out[0][same], out[1][same]) and all(same_bytes(x, y) for x, y in zip(one, two))
+        assert (out[0][9] == 0).all()
+        if store:
+            ops.qk_norm_rope_store8(qkv[4:5], *gains, None if cos_sin is None else cos_sin[4:5], i32([tables[4][32 // bs] * bs + 32 % bs]), q[4:5], *two,
+                                    H, KV, 1e-6)  # fmt: skip
+            ops.attn_single_query8(q, *two, order, positions, None, i32(tables), out[1], scale, window, 300, part_size=part)
+            assert torch.equal(out[0][4], out[1][4])
