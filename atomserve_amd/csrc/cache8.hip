@@ -647,58 +647,51 @@ struct Fresh {
   int store;    // 0: queries only, the block already holds the token
 };
 
-// The token's key and value (fp32, D each) into the operands of the step that holds it, its place in the step being `nth`, and with `write` into its block.
+// The token's key and value as its block holds them, in LDS.
+template <int D> struct News {
+  unsigned bytes[2][D / 4];
+  float scale[2];  // the block's, with the token
+  float by[2];     // what the block's other numbers are multiplied by: below 1 where the scale grows
+};
+
+// They go into the operands of the step that holds the token, its place in the step being `nth`, and with `write` into the block.
 template <int D>
-__device__ __forceinline__ void insert(Held<D>& held, const float* key, const float* value, int nth, const Pages& pages, unsigned block, bool write) {
+__device__ __forceinline__ void insert(Held<D>& held, const News<D>& news, int nth, const Pages& pages, unsigned block, bool write) {
   const int lane = threadIdx.x & (WAVE - 1), col = lane & 15, grp = lane >> 4, piece = nth >> 4, off = nth & 15;
-  float kmax = 0.f, vmax = 0.f;
-#pragma unroll
-  for (int i = 0; i < D / 64; ++i) {
-    kmax = fmaxf(kmax, fabsf(key[64 * i + lane]));
-    vmax = fmaxf(vmax, fabsf(value[64 * i + lane]));
-  }
-  auto before = [&](float scale) { return off > 0 ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scale), 16 * piece)) : 0.f; };
-  const float kold = before(held.ks), vold = before(held.vs);
-  const float kscale = fmaxf(kold, block_scale(wave_max(kmax))), vscale = fmaxf(vold, block_scale(wave_max(vmax)));
-  const float kinv = inverse_of(kscale), vinv = inverse_of(vscale);
-  const bool kgrows = kold > 0.f && kscale > kold, vgrows = vold > 0.f && vscale > vold;  // uniform
-  uint8_t* const krows = pages.k + (size_t)block * (BLOCK * D) + 16 * grp;
+  const float kby = news.by[0], vby = news.by[1];
   if (col >> 2 == piece) {  // this lane's keys are the block's
+    uint8_t* const rows = pages.k + (size_t)block * (BLOCK * D) + 16 * grp;
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) {
       const int row = 4 * tt + (col & 3);
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
-        if (kgrows)
+        if (kby < 1.f)  // uniform
 #pragma unroll
-          for (int w = 0; w < 4; ++w) held.k[tt][c][w] = rescale4(held.k[tt][c][w], kold * kinv);
-        if (row == off) {
-          const float* x = key + 64 * c + 16 * grp;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) held.k[tt][c][w] = pack4(x[4 * w] * kinv, x[4 * w + 1] * kinv, x[4 * w + 2] * kinv, x[4 * w + 3] * kinv);
-        }
-        if (write && (kgrows || row == off)) *reinterpret_cast<u32x4_t*>(krows + row * D + 64 * c) = held.k[tt][c];
+          for (int w = 0; w < 4; ++w) held.k[tt][c][w] = rescale4(held.k[tt][c][w], kby);
+        if (row == off) held.k[tt][c] = *reinterpret_cast<const u32x4_t*>(&news.bytes[0][16 * c + 4 * grp]);
+        if (write && (kby < 1.f || row == off)) *reinterpret_cast<u32x4_t*>(rows + row * D + 64 * c) = held.k[tt][c];
       }
     }
   }
   if (grp == piece) {
-    held.ks = kscale;
-    held.vs = vscale;
+    held.ks = news.scale[0];
+    held.vs = news.scale[1];
     const unsigned shift = 8 * (off & 3), byte = 0xffu << shift;
     u32x4_t* const vcol = reinterpret_cast<u32x4_t*>(pages.v + (size_t)block * (BLOCK * D)) + col;
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) {
-      const unsigned fresh = pack4(value[16 * d + col] * vinv, 0.f, 0.f, 0.f) << shift;
+      const unsigned fresh = (news.bytes[1][4 * d + (col >> 2)] >> (8 * (col & 3)) & 0xffu) << shift;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        if (vgrows) held.v[d][w] = rescale4(held.v[d][w], vold * vinv);
-        if (off >> 2 == w) held.v[d][w] = (held.v[d][w] & ~byte) | (fresh & byte);
+        if (vby < 1.f) held.v[d][w] = rescale4(held.v[d][w], vby);
+        if (off >> 2 == w) held.v[d][w] = (held.v[d][w] & ~byte) | fresh;
       }
       if (write) vcol[16 * d] = held.v[d];
     }
     if (write && col == 0) {
-      pages.ks[block] = kscale;
-      pages.vs[block] = vscale;
+      pages.ks[block] = held.ks;
+      pages.vs[block] = held.vs;
     }
   }
 }
@@ -707,7 +700,7 @@ __device__ __forceinline__ void insert(Held<D>& held, const float* key, const fl
 template <int D, bool FRESH, typename W>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a, Fresh fresh) {
   constexpr int LD = D + 4;
-  extern __shared__ __align__(16) float smem[];  // [4][16] m, [4][16] l, [4][G][LD]; FRESH: [2][D] key and value, [G][D + 8] bf16 queries
+  extern __shared__ __align__(16) float smem[];  // [4][16] m, [4][16] l, [4][G][LD]; FRESH: the news, [G][D + 8] bf16 queries
   const int G = a.H / a.KV, part = blockIdx.y, N = gridDim.x / a.KV;
   int item = blockIdx.x / a.KV, kvh = blockIdx.x - item * a.KV;
   if (a.P == 1) {
@@ -728,6 +721,19 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a
   const Pieces pieces{a.tables + (size_t)(a.tok_row ? a.tok_row[t] : t) * a.table_width, max(pos, 0) / BLOCK, a.magic};
   const Steps steps(lo, a.sight.keep, pos);
   const int from = part * a.part_steps, to = min(steps.count, from + a.part_steps);
+  [[maybe_unused]] const int last = steps.count - 1;  // the step that ends with the token's own position
+  [[maybe_unused]] const bool here = FRESH && fresh.store && last >= from && last < to;
+  [[maybe_unused]] unsigned own_block = 0;
+  [[maybe_unused]] bool write = false;  // whether the token is kept
+  if constexpr (FRESH) {
+    if (here) {
+      Blocks own;
+      own.ask(a.pages, pieces, pos);
+      const int slot = fresh.from.slots[t];
+      own_block = Blocks::of(a.pages, kvh, own.p0, own.s0);
+      write = slot >= 0 && slot / bs < a.pages.num_pages && block_index(a.pages, slot / bs, kvh, slot % bs / BLOCK) == own_block;
+    }
+  }
   // a step's operands are asked for a step ahead, where they lie two steps ahead
   Held<D> even, odd;
   Blocks blocks;
@@ -741,38 +747,49 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a
   Running<D> run;
   run.clear();
   Query<D> q;
-  [[maybe_unused]] float* const news = smem + 128 + 4 * LD * G;  // FRESH: the token's key and value
-  [[maybe_unused]] const int last = steps.count - 1;             // the step that ends with the token's own position
-  [[maybe_unused]] const bool here = FRESH && fresh.store && last >= from && last < to;
+  [[maybe_unused]] News<D>* const news = reinterpret_cast<News<D>*>(smem + 128 + 4 * LD * G);
   if constexpr (FRESH) {
     constexpr int LPT = Lanes<D>::LPT, AT_ONCE = Lanes<D>::AT_ONCE;
     const Append& f = fresh.from;
-    bf16* const queries = reinterpret_cast<bf16*>(news + 2 * D);
+    bf16* const queries = reinterpret_cast<bf16*>(news + 1);
     const int j = lane % LPT, jobs = G + (here ? 2 : 0), heads = a.H + 2 * a.KV;
     const bool busy = 8 * j < D;
     for (int job = wave * AT_ONCE + lane / LPT; job < jobs; job += 4 * AT_ONCE) {  // the group's queries, the key, the value; whole lane groups
       const bool query = job < G, key = job == G;
       const Places at8(busy ? j : 0, job <= G ? f.R : 0);
       const bf16* src = f.qkv + ((size_t)t * heads + (query ? h0 + job : a.H + kvh + (key ? 0 : a.KV))) * D;
-      float x[8], g[8];
+      float x[8], g[8], before = 0.f;
       load4(src + at8.a, x);
       load4(src + at8.b, x + 4);
+      if (!query && pos % BLOCK > 0) before = (key ? a.pages.ks : a.pages.vs)[own_block];  // a block that begins with this token is new
       const W* gains = (const W*)(query ? f.qw : f.kw);
       if (gains) {
         load4(gains + at8.a, g);
         load4(gains + at8.b, g + 4);
       }
       if (job <= G) norm_turn<D>(x, gains != nullptr, g, f.cs, f.eps, f.R, t, j, busy);
-      if (!busy) continue;
       if (query) {
+        if (!busy) continue;
         bf16* to8 = queries + job * (D + 8);
         *reinterpret_cast<bf16x4_t*>(to8 + at8.a) = bf16x4_t{(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]};
         *reinterpret_cast<bf16x4_t*>(to8 + at8.b) = bf16x4_t{(bf16)x[4], (bf16)x[5], (bf16)x[6], (bf16)x[7]};
       } else {
-        float* to8 = news + (key ? 0 : D);
+        float amax = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          to8[(i < 4 ? at8.a : at8.b - 4) + i] = __builtin_amdgcn_fmed3f(finite_or_zero(x[i]), -LARGEST * 0x1p119f, LARGEST * 0x1p119f);
+        for (int i = 0; i < 8; ++i) {
+          x[i] = __builtin_amdgcn_fmed3f(finite_or_zero(x[i]), -LARGEST * 0x1p119f, LARGEST * 0x1p119f);
+          amax = fmaxf(amax, fabsf(x[i]));
+        }
+        const float scale = fmaxf(before, block_scale(lanes_max<LPT>(amax))), inv = inverse_of(scale);
+        const int which = key ? 0 : 1;
+        if (busy) {
+          news->bytes[which][at8.a / 4] = pack4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+          news->bytes[which][at8.b / 4] = pack4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
+        }
+        if (j == 0) {
+          news->scale[which] = scale;
+          news->by[which] = before > 0.f ? before * inv : 1.f;
+        }
       }
     }
     __syncthreads();
@@ -784,12 +801,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a
   auto turn = [&](Held<D>& now, Held<D>& next) {
     if constexpr (FRESH) {
       if (here && at == last) {  // uniform: this wave's step holds the token itself
-        const int slot = fresh.from.slots[t];
-        Blocks own;
-        own.ask(a.pages, pieces, pos);
-        const unsigned block = Blocks::of(a.pages, page_head, own.p0, own.s0);
-        const bool write = slot >= 0 && slot / bs < a.pages.num_pages && block_index(a.pages, slot / bs, page_head, slot % bs / BLOCK) == block;
-        insert<D>(now, news, news + D, pos % STEP, a.pages, block, write);
+        insert<D>(now, *news, pos % STEP, a.pages, own_block, write);
       }
     }
     if (at + 4 < to) {
@@ -1286,14 +1298,14 @@ extern "C" int as_attn_single_query8(const void* q, const void* k_pages, const v
 
 // A decode step (token t is row t of the block tables, slots[t] the place of its own position there, or negative: attended, not kept) from the projection's
 // output qkv [T, H + 2 KV, D]: append and attention in one kernel.  items [T]: the order in which tokens are taken, or null; store 0: queries only.  At most 16
-// query heads to a kv head; window as everywhere; parts and part_size as for single queries.
+// query heads of at most 192 to a kv head; window as everywhere; parts and part_size as for single queries.
 extern "C" int as_attn_decode_fresh8(const void* qkv, const void* qw, const void* kw, int w_dtype, const float* cs, const int* slots, float eps,
                                      int store, void* k_pages, void* v_pages, float* k_scales, float* v_scales, int num_pages, const int* items,
                                      int num_tokens, const int* positions, const int* block_tables, int table_width, void* out, float* parts,
                                      int H, int KV, int D, int R, int bs, float scale, int window, int part_size, int P, hipStream_t stream) {
   if (num_tokens <= 0) return AS_OK;
   const Sight sight{window, 0, 0, 0.f, 0, nullptr, 0};
-  if (!sight_ok(sight) || H <= 0 || KV <= 0 || H % KV || H / KV > 16 || R < 0 || R > D || R % 8 || (R > 0) != (cs != nullptr)) return AS_BAD_SHAPE;
+  if (!sight_ok(sight) || H <= 0 || KV <= 0 || H % KV || H / KV > 16 || D > 192 || R < 0 || R > D || R % 8 || (R > 0) != (cs != nullptr)) return AS_BAD_SHAPE;
   if (!pages_ok(k_pages, v_pages, k_scales, v_scales, num_pages, KV, D, bs) || !table_ok(num_pages, KV, bs, table_width)) return AS_BAD_SHAPE;
   if (!qkv || (qw == nullptr) != (kw == nullptr) || (store && !slots) || !positions || !block_tables || !out) return AS_BAD_SHAPE;
   if (part_size <= 0 || part_size % STEP || P <= 0 || P > 65535 || (long long)num_tokens * KV > 0x7fffffffll) return AS_BAD_SHAPE;
@@ -1304,7 +1316,7 @@ extern "C" int as_attn_decode_fresh8(const void* qkv, const void* qw, const void
   const Attend a{nullptr, pages, items, positions, nullptr, nullptr, block_tables, table_width, (bf16*)out, parts + rows * D, parts + rows * (D + 1),
                  parts, H, KV, 1, scale, sight, part_size / STEP, P, magic_of(bs), compute_units()};
   const Fresh fresh{Append{(const bf16*)qkv, qw, kw, (const float2*)cs, slots, nullptr, pages, num_tokens, H, R, eps, 0, 0}, store};
-  const size_t shmem = sizeof(float) * (128 + 4 * (size_t)(D + 4) * (H / KV) + 2 * D) + sizeof(bf16) * (size_t)(D + 8) * (H / KV);
+  const size_t shmem = sizeof(float) * (128 + 4 * (size_t)(D + 4) * (H / KV) + 4) + 2 * (size_t)D + sizeof(bf16) * (size_t)(D + 8) * (H / KV);
 #define LAUNCH2(DV, W)                                                                                                                   \
   {                                                                                                                                      \
     const auto kernel = single8_kernel<DV, true, W>;                                                                                     \
@@ -1313,7 +1325,11 @@ extern "C" int as_attn_decode_fresh8(const void* qkv, const void* qw, const void
     kernel<<<dim3(KV * num_tokens, P), 256, shmem, stream>>>(a, fresh);                                                                  \
   }
 #define LAUNCH(DV) if (w_dtype == DT_F32) LAUNCH2(DV, float) else LAUNCH2(DV, bf16)
-  FOR_WIDTH(LAUNCH)
+  switch (D / 64) {
+    case 1: LAUNCH(64) break;
+    case 2: LAUNCH(128) break;
+    default: LAUNCH(192) break;
+  }
 #undef LAUNCH
 #undef LAUNCH2
   if (hipGetLastError() != hipSuccess) return AS_LAUNCH_FAILED;

@@ -954,6 +954,8 @@ def attn_single_query8(q, k_pages, v_pages, k_scales, v_scales, items, positions
     if items is not None:
         _check(items, "items", I32, (None,))
         N = items.shape[0]
+        if T == N == 1:  # it can only be token 0: a wait for memory less
+            items = None
     _good_or_check(positions, "positions", I32, (T,))
     if tok_row is not None:
         _good_or_check(tok_row, "tok_row", I32, (T,))
@@ -978,8 +980,15 @@ def attn_single_query8(q, k_pages, v_pages, k_scales, v_scales, items, positions
 
 
 def attn_decode_fresh8_supported(dtype, num_heads: int, num_kv_heads: int, head_dim: int, block_size: int, rotary_dim: int) -> bool:
-    """Whether `attn_decode_fresh8` takes this case: what `cache8_supported` names, at most 16 query heads to a kv head."""
-    return cache8_supported(dtype, num_heads, num_kv_heads, head_dim, block_size, rotary_dim) and num_heads // num_kv_heads <= 16
+    """Whether `attn_decode_fresh8` takes this case: what `cache8_supported` names, at most 16 query heads to a kv head, heads of up to 192.  us of the one
+    kernel / of the two, heads of 128 (32 on 8), 64 (16 on 4), 192 (24 on 8), by requests x tokens (heads of 256, 8 on 4, whose operands fill the registers:
+    10.6/10.3, 13.2/13.0, 15.6/17.5, 54.8/50.2, 45.5/37.7; not taken):
+        1 x 100       1 x 2,000     8 x 2,048     64 x 2,048    128 x 500
+        8.0/8.7       10.5/11.3     13.2/14.5     45.0/46.5     32.8/31.9
+        6.5/7.7       8.9/10.2      8.7/10.4      16.9/17.6     10.4/11.6
+        9.6/9.8       12.3/12.5     17.8/19.0     69.3/69.2     57.6/52.2"""
+    return (cache8_supported(dtype, num_heads, num_kv_heads, head_dim, block_size, rotary_dim) and num_heads // num_kv_heads <= 16
+            and head_dim <= 192)  # fmt: skip
 
 
 def attn_decode_fresh8(qkv, q_weight, k_weight, cos_sin, slots, eps, store_kv, k_pages, v_pages, k_scales, v_scales, positions, block_tables, out,
@@ -1015,6 +1024,8 @@ def attn_decode_fresh8(qkv, q_weight, k_weight, cos_sin, slots, eps, store_kv, k
         _good_or_check(slots, "slots", I32, (T,))
     if order is not None:
         _good_or_check(order, "order", I32, (T,))
+        if T == 1:
+            order = None
     if window < 0:
         raise KernelError("attention: a window is not negative")
     if T == 0:

@@ -126,6 +126,8 @@ def test_prompts_refuse(wrong):
     {"q_weight": lambda: tensor(64)}, {"positions": lambda: tensor(4, dtype=I32)}, {"order": lambda: tensor(2, dtype=I32)},
     {"block_tables": lambda: tensor(2, 4, dtype=I32)}, {"max_context": lambda: 65}, {"window": lambda: -1}, {"scale": lambda: 0.0},
     {"scale": lambda: -1.0}, {"part_size": lambda: 32},
+    {"qkv": lambda: tensor(3, 8, 256), "k_pages": lambda: tensor(4, 2, 16, 256, dtype=E4M3), "v_pages": lambda: tensor(4, 2, 1, 256, 16, dtype=E4M3),
+     "out": lambda: tensor(3, 4, 256), "cos_sin": lambda: tensor(3, 128, 2, dtype=F32)},  # two kernels are faster
     {"qkv": lambda: tensor(3, 34 + 4, 64), "num_heads": lambda: 34, "out": lambda: tensor(3, 34, 64)},  # 17 heads to a kv head
 ])  # fmt: skip
 def test_decode_steps_from_the_projection_refuse(wrong):
