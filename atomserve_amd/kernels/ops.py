@@ -808,32 +808,65 @@ def cache8_supported(dtype, num_heads: int, num_kv_heads: int, head_dim: int, bl
             and rotary_dim % 8 == 0)  # fmt: skip
 
 
-# The calls below are made once a layer and are as long as their Python where steps are not replayed: one expression per call looks at all that is usually
-# right, and `_check` says what is wrong where it is not (append of one token, host and launch: 14.5 us with a check per tensor).
+# The calls below are made once a layer and are as long as their Python where steps are not replayed: what is right passes in one expression a tensor, and
+# `_check` says what is wrong where it is not.
 
 
-def _good(t, dtype, shape) -> bool:
-    return t.dtype is dtype and t.shape == shape and t.is_cuda and t.is_contiguous()
+def _device() -> int:
+    return torch._C._cuda_getDevice()
 
 
-def _pages8(k_pages, v_pages, k_scales, v_scales, num_kv_heads=None) -> tuple:
-    """(pages, kv heads, tokens of a page, head width) of a cache in 8 bits."""
+def _check8(t, name, dtype, shape, here: int) -> None:
+    """`_check` of one dtype and a whole shape, and that the tensor lies on the current device, whose stream the kernel is put on."""
     try:
-        NB, KV, bs, D = shape = k_pages.shape
-        scales = (NB, KV, bs // BLOCK8)
-        good = (_good(k_pages, E4M3, shape) and _good(v_pages, E4M3, (*scales, D, BLOCK8)) and _good(k_scales, F32, scales)
-                and _good(v_scales, F32, scales) and KV == (num_kv_heads or KV))  # fmt: skip
-    except (AttributeError, ValueError):
-        good = False
-    if not good:
-        _check(k_pages, "k_pages", E4M3, (None, num_kv_heads, None, None))
-        NB, KV, bs, D = k_pages.shape
-        _check(v_pages, "v_pages", E4M3, (NB, KV, bs // BLOCK8, D, BLOCK8))
-        _check(k_scales, "k_scales", F32, (NB, KV, bs // BLOCK8))
-        _check(v_scales, "v_scales", F32, (NB, KV, bs // BLOCK8))
+        if t.dtype is dtype and t.shape == shape and t.get_device() == here and t.is_contiguous():
+            return
+    except AttributeError:  # no tensor
+        pass
+    _check(t, name, dtype, shape)
+    if t.get_device() != here:
+        raise KernelError(f"{name} lies on cuda:{t.get_device()}, the current device is cuda:{here}")
+
+
+def _shape8(t, name, dims: int) -> tuple:
+    """The shape of what has to be a tensor of `dims` dimensions."""
+    if not isinstance(t, torch.Tensor) or t.dim() != dims:
+        _check(t, name, None, (None,) * dims)
+    return t.shape
+
+
+def _pages8(k_pages, v_pages, k_scales, v_scales, here: int) -> tuple:
+    """(pages, kv heads, tokens of a page, head width) of a cache in 8 bits."""
+    NB, KV, bs, D = shape = _shape8(k_pages, "k_pages", 4)
+    scales = (NB, KV, bs // BLOCK8)
+    _check8(k_pages, "k_pages", E4M3, shape, here)
+    _check8(v_pages, "v_pages", E4M3, (*scales, D, BLOCK8), here)
+    _check8(k_scales, "k_scales", F32, scales, here)
+    _check8(v_scales, "v_scales", F32, scales, here)
     if bs % BLOCK8 or bs == 0 or D % 64 or not 0 < D <= 256 or NB == 0 or KV == 0:
         raise KernelError(f"a cache in 8 bits has pages of a multiple of {BLOCK8} tokens and heads of 64, 128, 192 or 256, not {bs} and {D}")
     return NB, KV, bs, D
+
+
+def _gains8(q_weight, k_weight, D: int, here: int):
+    """The dtype of a pair of gains [D], both or neither of them given."""
+    if q_weight is None and k_weight is None:
+        return BF16
+    if q_weight is None or k_weight is None:
+        raise KernelError("q and k norm weights come together")
+    dtype = F32 if getattr(q_weight, "dtype", None) is F32 else BF16
+    _check8(q_weight, "q_weight", dtype, (D,), here)
+    _check8(k_weight, "k_weight", dtype, (D,), here)
+    return dtype
+
+
+def _turn8(cos_sin, T: int, here: int) -> int:
+    """How many coordinates a table of angles turns."""
+    if cos_sin is None:
+        return 0
+    shape = _shape8(cos_sin, "cos_sin", 3)
+    _check8(cos_sin, "cos_sin", F32, (T, shape[1], 2), here)
+    return 2 * shape[1]
 
 
 def _addresses(*tensors) -> list:
@@ -841,12 +874,6 @@ def _addresses(*tensors) -> list:
     if watch.held is not None:
         return [_ptr(t) for t in tensors]
     return [0 if t is None else t.data_ptr() for t in tensors]
-
-
-def _good_or_check(t, name, dtype, shape) -> None:
-    """`_check` of one dtype and a shape without gaps."""
-    if not isinstance(t, torch.Tensor) or not _good(t, dtype, shape):
-        _check(t, name, dtype, shape)
 
 
 def qk_norm_rope_store8(qkv, q_weight, k_weight, cos_sin, slots, q_out, k_pages, v_pages, k_scales, v_scales, num_heads, num_kv_heads, eps,
@@ -857,28 +884,20 @@ def qk_norm_rope_store8(qkv, q_weight, k_weight, cos_sin, slots, q_out, k_pages,
     qkv [T, H + 2 KV, D], q_out [T, H, D] bfloat16; slots [T] int32 (page * block_size + offset, or -1 for a token whose keys are not stored; one
     beyond the pages stores nothing either).  The tokens that go into one block come as one run, next to each other and in the order of their places, as a request's
     tokens do: two runs of one call in one block, or one place twice, leave that block undefined.  What is not finite is stored as zero."""
-    _check(qkv, "qkv", BF16, (None, num_heads + 2 * num_kv_heads, None))
-    T, _, D = qkv.shape
-    _good_or_check(q_out, "q_out", BF16, (T, num_heads, D))
-    R = 0
-    if cos_sin is not None:
-        _check(cos_sin, "cos_sin", F32, (T, None, 2))
-        R = 2 * cos_sin.shape[1]
+    here = _device()
+    T, _, D = _shape8(qkv, "qkv", 3)
+    _check8(qkv, "qkv", BF16, (T, num_heads + 2 * num_kv_heads, D), here)
+    _check8(q_out, "q_out", BF16, (T, num_heads, D), here)
+    R = _turn8(cos_sin, T, here)
     if R > D or R % 8 or D % 64 or not 0 < D <= 256:
         raise KernelError(f"appending in 8 bits: unsupported head width {D} (64, 128, 192 or 256) or rotary width {R} (a multiple of 8)")
-    w_dtype = BF16
-    if q_weight is not None and k_weight is not None:
-        _check(q_weight, "q_weight", (F32, BF16), (D,))
-        w_dtype = q_weight.dtype
-        _good_or_check(k_weight, "k_weight", w_dtype, (D,))
-    elif q_weight is not None or k_weight is not None:
-        raise KernelError("q and k norm weights come together")
+    w_dtype = _gains8(q_weight, k_weight, D, here)
     NB, bs, cache = 1, BLOCK8, (None,) * 5
     if store_kv:
-        _good_or_check(slots, "slots", I32, (T,))
-        NB, _, bs, width = _pages8(k_pages, v_pages, k_scales, v_scales, num_kv_heads)
-        if width != D:
-            raise KernelError(f"k_pages has heads of {width}, qkv of {D}")
+        _check8(slots, "slots", I32, (T,), here)
+        NB, KV, bs, width = _pages8(k_pages, v_pages, k_scales, v_scales, here)
+        if KV != num_kv_heads or width != D:
+            raise KernelError(f"k_pages has {KV} heads of {width}, qkv {num_kv_heads} of {D}")
         cache = slots, k_pages, v_pages, k_scales, v_scales
     p_qkv, p_qw, p_kw, p_cs, p_q, p_slots, *pages = _addresses(qkv, q_weight, k_weight, cos_sin if R else None, q_out, *cache)
     call("as_qk_norm_rope_store8", p_qkv, p_qw, p_kw, _DT[w_dtype], p_cs, p_slots, p_q, *pages, NB, T, num_heads, num_kv_heads, D, R, float(eps), bs,
@@ -946,21 +965,24 @@ def _share8(group: int) -> int:
 def attn_single_query8(q, k_pages, v_pages, k_scales, v_scales, items, positions, tok_row, block_tables, out, scale, window, max_context,
                        part_size=None, keep_first=0, softcap=0.0, sink=False, chunk=0) -> None:  # fmt: skip
     """`attn_single_query` of bfloat16 heads over a cache in 8 bits: arguments as there.  A query at a negative position sees nothing: zeros."""
-    _check(q, "q", BF16, (None, None, None))
-    T, H, D = q.shape
+    here = _device()
+    T, H, D = shape = _shape8(q, "q", 3)
+    _check8(q, "q", BF16, shape, here)
     sight = _sight(window, keep_first, chunk, softcap, sink, q, out)
-    NB, KV, bs, width = _pages8(k_pages, v_pages, k_scales, v_scales)
+    if out.get_device() != here or (sight[5] and sink.get_device() != here):
+        raise KernelError(f"attention over 8 bits: results or sinks lie on another device than the current one, cuda:{here}")
+    NB, KV, bs, width = _pages8(k_pages, v_pages, k_scales, v_scales, here)
     N = T
     if items is not None:
-        _check(items, "items", I32, (None,))
-        N = items.shape[0]
+        N, = _shape8(items, "items", 1)
+        _check8(items, "items", I32, (N,), here)
         if T == N == 1:  # it can only be token 0: a wait for memory less
             items = None
-    _good_or_check(positions, "positions", I32, (T,))
+    _check8(positions, "positions", I32, (T,), here)
     if tok_row is not None:
-        _good_or_check(tok_row, "tok_row", I32, (T,))
-    _check(block_tables, "block_tables", I32, (None, None))
-    rows, table_width = block_tables.shape
+        _check8(tok_row, "tok_row", I32, (T,), here)
+    rows, table_width = _shape8(block_tables, "block_tables", 2)
+    _check8(block_tables, "block_tables", I32, (rows, table_width), here)
     if tok_row is None and rows < T:
         raise KernelError(f"attention: {T} tokens that are their own rows need as many block tables")
     if N == 0:
@@ -996,34 +1018,26 @@ def attn_decode_fresh8(qkv, q_weight, k_weight, cos_sin, slots, eps, store_kv, k
     """`attn_decode_fresh` over a cache in 8 bits: what `qk_norm_rope_store8` and then `attn_single_query8` do for tokens that are their own rows (token t
     reads block table t), in one kernel and with the same numbers; the per-head norm and the rotation may be missing.  slots[t] is the place that block
     table t names for positions[t], or negative: the token is attended and not kept."""
-    _check(qkv, "qkv", BF16, (None, None, None))
-    T, heads, D = qkv.shape
+    here = _device()
+    T, heads, D = shape = _shape8(qkv, "qkv", 3)
+    _check8(qkv, "qkv", BF16, shape, here)
     H = num_heads
-    NB, KV, bs, width = _pages8(k_pages, v_pages, k_scales, v_scales)
-    R = 0
-    if cos_sin is not None:
-        _check(cos_sin, "cos_sin", F32, (T, None, 2))
-        R = 2 * cos_sin.shape[1]
+    NB, KV, bs, width = _pages8(k_pages, v_pages, k_scales, v_scales, here)
+    R = _turn8(cos_sin, T, here)
     if heads != H + 2 * KV or width != D or R > D or not attn_decode_fresh8_supported(BF16, H, KV, D, bs, R):
         raise KernelError(f"attention from fresh projections over 8 bits: unsupported heads {H}/{KV} of {heads} in qkv, head width {D} ({width} in the "
                           f"pages) or rotary width {R}")  # fmt: skip
-    _good_or_check(out, "out", BF16, (T, H, D))
-    _good_or_check(positions, "positions", I32, (T,))
-    _check(block_tables, "block_tables", I32, (None, None))
-    rows, table_width = block_tables.shape
+    _check8(out, "out", BF16, (T, H, D), here)
+    _check8(positions, "positions", I32, (T,), here)
+    rows, table_width = _shape8(block_tables, "block_tables", 2)
+    _check8(block_tables, "block_tables", I32, (rows, table_width), here)
     if rows < T:
         raise KernelError(f"attention: {T} tokens that are their own rows need as many block tables")
-    w_dtype = BF16
-    if q_weight is not None and k_weight is not None:
-        _check(q_weight, "q_weight", (F32, BF16), (D,))
-        w_dtype = q_weight.dtype
-        _good_or_check(k_weight, "k_weight", w_dtype, (D,))
-    elif q_weight is not None or k_weight is not None:
-        raise KernelError("q and k norm weights come together")
+    w_dtype = _gains8(q_weight, k_weight, D, here)
     if store_kv:
-        _good_or_check(slots, "slots", I32, (T,))
+        _check8(slots, "slots", I32, (T,), here)
     if order is not None:
-        _good_or_check(order, "order", I32, (T,))
+        _check8(order, "order", I32, (T,), here)
         if T == 1:
             order = None
     if window < 0:
@@ -1088,13 +1102,17 @@ def _prefill8_plan(num_tiles, H, KV, D, max_context, window, query_tiles, tile_k
 def attn_prefill8(q, k_pages, v_pages, k_scales, v_scales, tiles, block_tables, out, scale, window, max_context, query_tiles=None,
                   tile_keys: int = 0, keep_first=0, softcap=0.0, sink=False, chunk=0) -> None:  # fmt: skip
     """`attn_prefill` over a cache in 8 bits: arguments as there."""
-    _check(q, "q", BF16, (None, None, None))
-    T, H, D = q.shape
+    here = _device()
+    T, H, D = shape = _shape8(q, "q", 3)
+    _check8(q, "q", BF16, shape, here)
     sight = _sight(window, keep_first, chunk, softcap, sink, q, out)
-    NB, KV, bs, width = _pages8(k_pages, v_pages, k_scales, v_scales)
-    _check(tiles, "tiles", I32, (None, 4))
-    _check(block_tables, "block_tables", I32, (None, None))
-    num_tiles, table_width = tiles.shape[0], block_tables.shape[1]
+    if out.get_device() != here or (sight[5] and sink.get_device() != here):
+        raise KernelError(f"attention over 8 bits: results or sinks lie on another device than the current one, cuda:{here}")
+    NB, KV, bs, width = _pages8(k_pages, v_pages, k_scales, v_scales, here)
+    num_tiles, _ = _shape8(tiles, "tiles", 2)
+    _check8(tiles, "tiles", I32, (num_tiles, 4), here)
+    rows, table_width = _shape8(block_tables, "block_tables", 2)
+    _check8(block_tables, "block_tables", I32, (rows, table_width), here)
     if num_tiles == 0:
         return
     if H % KV or width != D:

@@ -17,6 +17,7 @@ def nothing_is_launched(monkeypatch):
     monkeypatch.setattr(ops, "call", call)
     monkeypatch.setattr(ops, "_addresses", lambda *tensors: [0] * len(tensors))
     monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(ops, "_device", lambda: 0)
     monkeypatch.setattr(ops, "_compute_units", 256)
     with FakeTensorMode():  # tensors that say they are on the GPU, without memory
         yield
@@ -133,6 +134,22 @@ def test_prompts_refuse(wrong):
 def test_decode_steps_from_the_projection_refuse(wrong):
     with pytest.raises(ops.KernelError):
         fresh(**{k: v() for k, v in wrong.items()})
+
+
+@pytest.mark.parametrize("call,name", [(append, "qkv"), (append, "k_scales"), (single, "block_tables"), (prompt, "tiles"), (fresh, "slots")])
+def test_tensors_on_another_device_are_refused(monkeypatch, call, name):
+    """The kernel goes on the current device's stream."""
+    with pytest.raises(AssertionError, match="would have been launched") as launched:
+        call()
+    del launched
+    monkeypatch.setattr(ops, "_device", lambda: 1)
+    with pytest.raises(ops.KernelError, match="current device is cuda:1"):
+        call()
+    monkeypatch.setattr(ops, "_device", lambda: 0)
+    shapes = {"qkv": (3, 8, 64), "k_scales": (4, 2, 1), "block_tables": (3, 4), "tiles": (2, 4), "slots": (3,)}
+    dtype = {"qkv": BF16, "k_scales": F32}.get(name, I32)
+    with pytest.raises(ops.KernelError, match=f"{name} lies on cuda:1"):
+        call(**{name: torch.empty(shapes[name], dtype=dtype, device="cuda:1")})
 
 
 def test_nothing_to_do_launches_nothing():
