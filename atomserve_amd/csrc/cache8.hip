@@ -62,6 +62,9 @@ __device__ __forceinline__ size_t block_index(const Pages& p, int page, int kvh,
 // one kv head's keys or values; single tokens several at once, longer runs one after the other.  A run: tokens next to each other in the step that go to places next to each other of one block, so that one wave sees
 // all that the step puts there: the largest magnitude, the scale, and what the block held.  Lane group s has the run's places PASSES s .. + PASSES - 1 of the
 // block, so that a coordinate's bytes are neighbours in a lane's hands: they cross to the transposed block through LDS.
+//
+// Bound by memory where there is much of it (a prompt of 2,048 tokens, 32 heads of 128 on 8: 11.4 us, 47 MB at 4.2 TB/s; 16-bit pages 12.7) and by a launch
+// and three dependent waits (slots, scale, stores) where there is not: one token 2.9 us, 64 requests' tokens 4.7, 2.6 of it the queries.
 template <int D> struct Lanes {
   static constexpr int LPT = D <= 64 ? 8 : D <= 128 ? 16 : 32;  // lanes of a head, D / 8 of them busy
   static constexpr int AT_ONCE = WAVE / LPT, PASSES = BLOCK / AT_ONCE;
@@ -411,16 +414,18 @@ template <int D> struct Query {
 };
 
 template <int D> __device__ __forceinline__ void load_query(Query<D>& q, const bf16* row, int grp) {
-  float x[D / 64][16], amax = 0.f;
+  float x[D / 64][16];
+  unsigned most = 0;  // the largest magnitude's bits: of a query that is not finite those of an infinity or more
 #pragma unroll
   for (int c = 0; c < D / 64; ++c)
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
       load4(row + 64 * c + 16 * grp + i, x[c] + i);
 #pragma unroll
-      for (int n = 0; n < 4; ++n) amax = fmaxf(amax, fabsf(x[c][i + n]));
+      for (int n = 0; n < 4; ++n) most = max(most, __float_as_uint(x[c][i + n]) & 0x7fffffffu);
     }
-  q.scale = block_scale(quad_rows_max(amax));
+  const float amax = quad_rows_max(__uint_as_float(min(most, 0x7f800000u)));
+  q.scale = block_scale(amax);
   const float inv = inverse_of(q.scale);
 #pragma unroll
   for (int c = 0; c < D / 64; ++c)
@@ -434,6 +439,7 @@ template <int D> __device__ __forceinline__ void load_query(Query<D>& q, const b
       q.high[c][w] = high;
       q.low[c][w] = pack4(y[0] - a[0], y[1] - a[1], y[2] - b[0], y[3] - b[1]);
     }
+  if (amax == __builtin_inff()) q.scale = __builtin_nanf("");  // no e4m3 number stands for it: what it sees becomes NaN, and none of its neighbours
 }
 
 __device__ __forceinline__ i32x8_t both(u32x4_t a, u32x4_t b) {
@@ -697,6 +703,14 @@ __device__ __forceinline__ void insert(Held<D>& held, const News<D>& news, int n
 }
 
 // One workgroup per (token, group of query heads, partition of its keys); its four waves take the steps in turn.  W: of FRESH, the gains' type.
+//
+// Bound by the pages' bytes as soon as there are enough of them: 64 contexts of 300 to 8,000 tokens (32 heads of 128 on 8) 80 to 82 us, 6.5 TB/s (a large
+// copy reads and writes 5.1); one of 131,005 (64 heads on 8) 47 us with its merge, 5.7 TB/s.  16-bit pages: 182 and 85.  A step's operands go from memory into
+// registers in the order in which the matrix instructions take them: LDS would hold the same bytes once more, and nobody shares them, since all heads of a
+// group are columns of one wave.  Two steps in flight a wave (one being taken, one on its way) hide most of the latency: the
+// form that loaded a step when it came to it took 252 us for the 64 contexts.
+// Where there is little to read, latency is the bound: 700 keys of one request 7.1 us (16-bit pages 6.6), of which a launch, the page's entry, the
+// operands and the exchange between waves wait for one another.
 template <int D, bool FRESH, typename W>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a, Fresh fresh) {
   constexpr int LD = D + 4;
@@ -883,6 +897,12 @@ __global__ __launch_bounds__(256) void single8_merge_kernel(Attend a, int D) {
 //            slot (2 block + h) D + d holds keys 8 h .. + 7 of coordinate d, so that 16 lanes read 256 bytes in one piece.
 //
 // One barrier a round.  Where the blocks lie and their scales are looked up for 16 rounds at a time, a block a lane.
+//
+// Bound by what a SIMD issues: of a wave's round with QT 2 and heads of 128 the matrix cores are busy 1,026 cycles and the vector unit 1,283 (softmax, widening),
+// and the two waves of a SIMD take their sum, since a wave's products wait for its softmax.  2,048 tokens behind
+// 14,336 (32 heads on 8): 484 to 492 us, 1,050 TFLOP/s where an 8192^3 bf16 product reaches 1,212; 16-bit pages 522 to 537.  Keys read by every wave from memory, without LDS,
+// took 1,561.  A ring of four rounds in LDS was 3 to 20 per cent slower (room for fewer workgroups), a round's weighted values under the next
+// round's softmax 15 (spills), wave priorities no different.
 //
 // A step of few work items takes as long as its longest one: with `pieces` > 1 an item comes as that many workgroups, an item of more than `piece_rounds`
 // rounds is cut along its keys, and what the pieces leave (maxima, sums, unnormalised outputs) is put together by a second kernel.
@@ -1209,9 +1229,10 @@ __global__ __launch_bounds__(256) void prompt8_merge_kernel(Attend a, int units_
   }
 }
 
+template <typename... T> bool on_16_bytes(const T*... p) { return !(((uintptr_t)p | ...) & 15); }
 bool pages_ok(const void* k, const void* v, const float* ks, const float* vs, int num_pages, int KV, int D, int bs) {
   return k && v && ks && vs && num_pages > 0 && KV > 0 && D > 0 && D % 64 == 0 && D <= 256 && bs > 0 && bs % BLOCK == 0 &&
-         !(((uintptr_t)k | (uintptr_t)v) & 15);
+         on_16_bytes(k, v);
 }
 // ceil(2^32 / blocks of a page); a page of one block needs none
 unsigned magic_of(int bs) { return bs > BLOCK ? (unsigned)((0x100000000ull + bs / BLOCK - 1) / (bs / BLOCK)) : 0u; }
@@ -1242,10 +1263,13 @@ extern "C" int as_qk_norm_rope_store8(const void* qkv, const void* qw, const voi
                                       int H, int KV, int D, int R, float eps, int bs, int store, hipStream_t stream) {
   if (num_tokens <= 0) return AS_OK;
   if (H <= 0 || KV <= 0 || D <= 0 || D % 64 || D > 256 || R < 0 || R > D || R % 8 || (R > 0) != (cs != nullptr)) return AS_BAD_SHAPE;
-  if ((qw == nullptr) != (kw == nullptr) || !qkv || !q_out) return AS_BAD_SHAPE;
+  if ((qw == nullptr) != (kw == nullptr) || !qkv || !q_out || !on_16_bytes(qkv, qw, kw, cs, q_out)) return AS_BAD_SHAPE;
   if (store && (!slots || !pages_ok(k_pages, v_pages, k_scales, v_scales, num_pages, KV, D, bs))) return AS_BAD_SHAPE;
   if (w_dtype != DT_F32 && w_dtype != DT_BF16) return AS_BAD_DTYPE;
   if (R == 0) cs = nullptr;
+  // Tokens whose runs a wave takes: 16 is a block, so that a prompt's waves have one run each; with few (token, kv head) pairs compute units would stay
+  // empty.  us with 4 / with 16, 32 heads of 128 on 8: single tokens of 64 requests 4.7 / 9.2, of 256 6.4 / 11.1; prompts of 512 5.5 / 5.0, of 2,048
+  // 17.5 / 11.9, of 8,192 61.7 / 38.6.
   const int chunk = (long long)num_tokens * KV <= 2048 ? 4 : 16;
   const long long kv_blocks = store ? (((long long)num_tokens + chunk - 1) / chunk * 2 * KV + 3) / 4 : 0;
   const Append a{(const bf16*)qkv, qw, kw, (const float2*)cs, slots, (bf16*)q_out, pages_of(k_pages, v_pages, k_scales, v_scales, num_pages, KV, bs),
@@ -1274,9 +1298,9 @@ extern "C" int as_attn_single_query8(const void* q, const void* k_pages, const v
   const Sight sight{window, keep, chunk, cap, sink, sinks, wide};
   if (!sight_ok(sight) || H <= 0 || KV <= 0 || H % KV || H / KV > 16 || share < 1 || KV % share) return AS_BAD_SHAPE;
   if (!pages_ok(k_pages, v_pages, k_scales, v_scales, num_pages, KV / share, D, bs) || !table_ok(num_pages, KV / share, bs, table_width)) return AS_BAD_SHAPE;
-  if (!q || !positions || !block_tables || !out || part_size <= 0 || part_size % STEP || P <= 0 || P > 65535 || (long long)num_items * KV > 0x7fffffffll)
+  if (!q || !positions || !block_tables || !out || !on_16_bytes(q, out, parts) || part_size <= 0 || part_size % STEP || P <= 0 || P > 65535 || (long long)num_items * KV > 0x7fffffffll)
     return AS_BAD_SHAPE;
-  if (P > 1 && (!parts || (uintptr_t)parts & 15)) return AS_BAD_SHAPE;
+  if (P > 1 && !parts) return AS_BAD_SHAPE;
   const size_t rows = P > 1 ? (size_t)num_items * H * P : 0;
   const Attend a{(const bf16*)q, pages_of(k_pages, v_pages, k_scales, v_scales, num_pages, KV / share, bs), items, positions, tok_row, nullptr,
                  block_tables, table_width, (bf16*)out, parts + rows * D, parts + rows * (D + 1), parts, H, KV, share, scale, sight, part_size / STEP, P,
@@ -1307,9 +1331,10 @@ extern "C" int as_attn_decode_fresh8(const void* qkv, const void* qw, const void
   const Sight sight{window, 0, 0, 0.f, 0, nullptr, 0};
   if (!sight_ok(sight) || H <= 0 || KV <= 0 || H % KV || H / KV > 16 || D > 192 || R < 0 || R > D || R % 8 || (R > 0) != (cs != nullptr)) return AS_BAD_SHAPE;
   if (!pages_ok(k_pages, v_pages, k_scales, v_scales, num_pages, KV, D, bs) || !table_ok(num_pages, KV, bs, table_width)) return AS_BAD_SHAPE;
-  if (!qkv || (qw == nullptr) != (kw == nullptr) || (store && !slots) || !positions || !block_tables || !out) return AS_BAD_SHAPE;
+  if (!qkv || (qw == nullptr) != (kw == nullptr) || (store && !slots) || !positions || !block_tables || !out || !on_16_bytes(qkv, qw, kw, cs, out, parts))
+    return AS_BAD_SHAPE;
   if (part_size <= 0 || part_size % STEP || P <= 0 || P > 65535 || (long long)num_tokens * KV > 0x7fffffffll) return AS_BAD_SHAPE;
-  if (P > 1 && (!parts || (uintptr_t)parts & 15)) return AS_BAD_SHAPE;
+  if (P > 1 && !parts) return AS_BAD_SHAPE;
   if (w_dtype != DT_F32 && w_dtype != DT_BF16) return AS_BAD_DTYPE;
   const size_t rows = P > 1 ? (size_t)num_tokens * H * P : 0;
   const Pages pages = pages_of(k_pages, v_pages, k_scales, v_scales, num_pages, KV, bs);
@@ -1350,9 +1375,9 @@ extern "C" int as_attn_prefill8(const void* q, const void* k_pages, const void* 
   const Sight sight{window, keep, chunk, cap, sink, sinks, wide};
   if (!sight_ok(sight) || H <= 0 || KV <= 0 || H % KV || (query_tiles != 1 && query_tiles != 2)) return AS_BAD_SHAPE;
   if (!pages_ok(k_pages, v_pages, k_scales, v_scales, num_pages, KV, D, bs) || !table_ok(num_pages, KV, bs, table_width)) return AS_BAD_SHAPE;
-  if (!q || !tiles || !block_tables || !out) return AS_BAD_SHAPE;
+  if (!q || !tiles || !block_tables || !out || !on_16_bytes(q, out, parts)) return AS_BAD_SHAPE;
   if (pieces < 1) pieces = 1;
-  if (pieces > 1 && (piece_rounds < 1 || !parts || (uintptr_t)parts & 15 || tokens <= 0)) return AS_BAD_SHAPE;
+  if (pieces > 1 && (piece_rounds < 1 || !parts || tokens <= 0)) return AS_BAD_SHAPE;
   const int units_z = (64 / (16 * query_tiles) * (H / KV) + 3) / 4;
   const long long items = (long long)num_tiles * KV * units_z;
   if (items * pieces > 0x7fffffffll) return AS_BAD_SHAPE;

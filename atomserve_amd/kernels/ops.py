@@ -793,8 +793,9 @@ def attn_mixed(q, k_pages, v_pages, items, tiles, positions, tok_row, block_tabl
 #   v_pages  [num_pages, KV, block_size / 16, D, 16]    float8_e4m3fn (a block's values are transposed)
 #   k_scales, v_scales  [num_pages, KV, block_size / 16]  fp32
 #
-# Slots and block tables are those of a 16-bit cache.  What a block holds is known once its first place is written: a call that writes the first place
-# makes the block new and forgets what it held, and a call that goes on in a block lets its scale grow and rewrites it.  Pools start zeroed.
+# Slots and block tables are those of a 16-bit cache.  Blocks start on 16 bytes, as do the other tensors of these calls.  What a block holds is known once its first place is written: a call that writes the first place
+# makes the block new and forgets what it held, and a call that goes on in a block lets its scale grow and rewrites it.  Pools start zeroed
+# (what a mask hides is multiplied by zero, so it has to be a number): what is not finite is never stored.  A query that is not finite gives NaN.
 
 E4M3 = torch.float8_e4m3fn
 BLOCK8 = 16  # tokens that share a scale
@@ -1017,7 +1018,7 @@ def attn_decode_fresh8(qkv, q_weight, k_weight, cos_sin, slots, eps, store_kv, k
                        num_heads, scale, window, max_context, part_size=None, order=None) -> None:  # fmt: skip
     """`attn_decode_fresh` over a cache in 8 bits: what `qk_norm_rope_store8` and then `attn_single_query8` do for tokens that are their own rows (token t
     reads block table t), in one kernel and with the same numbers; the per-head norm and the rotation may be missing.  slots[t] is the place that block
-    table t names for positions[t], or negative: the token is attended and not kept."""
+    table t names for positions[t], or negative: the token is attended and not kept.  No two tokens are kept in one block, and `order` names each token once."""
     here = _device()
     T, heads, D = shape = _shape8(qkv, "qkv", 3)
     _check8(qkv, "qkv", BF16, shape, here)

@@ -232,3 +232,54 @@ def test_the_command_line_names_the_cache():
     assert build_parser().parse_args(["m"]).cache_bits == 0 and build_parser().parse_args(["m", "--cache-bits", "8"]).cache_bits == 8
     with pytest.raises(SystemExit):
         build_parser().parse_args(["m", "--cache-bits", "4"])
+
+
+# ---- how work is cut ------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("D", [64, 128, 192, 256])
+@pytest.mark.parametrize("KV,group", [(1, 1), (8, 4), (4, 24), (3, 7)])
+def test_partitions_cover_what_is_seen(D, KV, group):
+    share = ops._share8(group)
+    assert group % share == 0 and group // share <= 16 and all(group % n or group // n > 16 for n in range(1, share))
+    H = KV * group
+    for N in (1, 2, 9, 64, 500):
+        for context in (1, 63, 64, 65, 1000, 33_333, 1_000_000):
+            for window, keep in ((0, 0), (1, 0), (200, 0), (200, 70), (5000, 1)):
+                part, P, workspace = ops._partitions8(N, H, KV * share, D, context, window, None, "cuda:0", keep)
+                # no query walks more steps of 64 keys than this: all of them, or those that hold kept keys and those that the window reaches into
+                steps = -(-context // 64) if not window else min(-(-context // 64), -(-keep // 64) + (window - 1 + 63) // 64 + 1)
+                assert part % 64 == 0 and P * (part // 64) >= steps and 1 <= P <= 65535
+                assert (P == 1) == (workspace is None) and (P == 1 or workspace.numel() == N * H * P * (D + 2))
+                if N * KV * share >= 384:
+                    assert P == 1
+                assert ops.contexts_cut8(N, H, KV, D, context, window, keep) == (P > 1)
+
+
+def test_a_lone_long_context_is_cut_for_the_whole_gpu():
+    part, P, _ = ops._partitions8(1, 32, 8, 128, 131_072, 0, None, "cuda:0")
+    assert P * 8 >= 256 and part >= 256
+    assert ops._partitions8(1, 32, 8, 128, 100, 0, None, "cuda:0")[1] == 1
+    with pytest.raises(ops.KernelError, match="multiples of 64"):
+        ops._partitions8(1, 32, 8, 128, 100, 0, 96, "cuda:0")
+
+
+@pytest.mark.parametrize("D", [64, 128, 192, 256])
+@pytest.mark.parametrize("H,KV", [(32, 8), (4, 4), (24, 1)])
+def test_pieces_of_a_portion_cover_its_rounds(D, H, KV):
+    for tiles in (1, 2, 32, 300):
+        for context in (1, 64, 65, 2000, 100_000):
+            for window in (0, 100):
+                for forced in (None, 1, 3, 100):
+                    if context < 64 * (tiles - 1) / 16:
+                        continue
+                    kind, pieces, rounds = ops._prefill8_plan(tiles, H, KV, D, context, window, None, 0, forced, 256)
+                    span = min(context, window + 64) if window else context
+                    assert kind in (1, 2) and pieces >= 1
+                    if pieces > 1:
+                        assert pieces * rounds >= -(-span // 64) and rounds * 64 * pieces < 2 * span + 64 * pieces and (forced is None or pieces <= forced)
+
+
+def test_a_portion_behind_a_long_prefix_is_cut_and_many_are_not():
+    assert ops._prefill8_plan(1, 32, 8, 128, 16_000, 0, None, 0, None, 256)[1] > 1
+    assert ops._prefill8_plan(200, 32, 8, 128, 2_000, 0, None, 0, None, 256)[1] == 1
