@@ -462,9 +462,14 @@ template <int D> __device__ __forceinline__ f32x4_t score_tile(const u32x4_t (&k
   return s;
 }
 
+// What scores are taken relative to need not be their maximum: weights of up to 2^8 are as exact as those of up to 1.  So a maximum that has grown by less
+// moves nothing, and whether one has grown by more is all that a step asks; lanes agree on a new one, and sums are rescaled, only then.  (2,048 tokens behind
+// 14,336: 538 -> 493 us, ones in use as they were; wide heads and short portions alike.)
+constexpr float SLACK = 8.f;
+
 template <int D> struct Running {
   f32x4_t o[D / 16];
-  float m, l;  // the column's maximum (base 2), and the sum of this lane's weights
+  float m, l;  // the column's maximum (base 2) or up to SLACK less, and the sum of this lane's weights
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) o[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -568,8 +573,16 @@ __device__ __forceinline__ void take_step(const Held<D>& held, int kb, const Que
         s[tt][r] = key <= pos && (key >= lo || key < keep) ? s[tt][r] : NEG_INF;
       }
   }
-  const float mn = fmaxf(run.m, quad_rows_max(max_of_16(s) * by)), base = mn == NEG_INF ? 0.f : mn;
-  const float alpha = __builtin_amdgcn_exp2f(run.m - base);
+  const float top = max_of_16(s) * by;
+  if (__any(top > run.m + SLACK)) {  // uniform; rare once the first keys have been seen
+    const float mn = fmaxf(run.m, quad_rows_max(top));
+    const float alpha = __builtin_amdgcn_exp2f(run.m - (mn == NEG_INF ? 0.f : mn));
+    run.m = mn;
+    run.l *= alpha;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) run.o[d] *= alpha;
+  }
+  const float base = run.m == NEG_INF ? 0.f : run.m;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
   bf16x8_t p[2];
 #pragma unroll
@@ -580,12 +593,7 @@ __device__ __forceinline__ void take_step(const Held<D>& held, int kb, const Que
       sum[r] += w;
       p[tt >> 1][(tt & 1) * 4 + r] = (bf16)w;
     }
-  run.m = mn;
-  run.l = run.l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-  if (__any(alpha != 1.f)) {
-#pragma unroll
-    for (int d = 0; d < D / 16; ++d) run.o[d] *= alpha;
-  }
+  run.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
   for (int d = 0; d < D / 16; ++d) {
     bf16x8_t v[2];
@@ -985,8 +993,15 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt8_kernel(Attend a
   Running<D> run[QT];
   int qpos[QT], qlo[QT];
   float factor[QT];
+  float base[QT];  // the columns' maxima; 0 while there is none
+  f32x4_t l[QT];  // sums of weights, the same in every row: the weights' product with ones
+  bf16x8_t ones;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ones[i] = (bf16)1.f;
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
+    l[qt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    base[qt] = 0.f;
     const int qc = min(qt * 16 + col, nq - 1);  // columns past the end repeat the last query and are not stored
     qpos[qt] = min(pos0 + q0 + qc, end);
     qlo[qt] = first_seen(qpos[qt]);
@@ -1094,18 +1109,18 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt8_kernel(Attend a
       __builtin_amdgcn_sched_barrier(0);
       const bool masked = kb + STEP - 1 > my_first || kb < last_lo;
       bf16x8_t p[QT][2];
-      float alpha[QT];
-      bool rescale = false;
+      float by[QT], top[QT];  // top: the largest score of this lane's 16
+      bool grows = false;
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
-        float by = factor[qt] * fmaxf(ks, 0x1p-100f);
+        by[qt] = factor[qt] * fmaxf(ks, 0x1p-100f);
         if (a.sight.cap > 0.f) {
-          by *= __builtin_amdgcn_rcpf(a.sight.cap);
+          by[qt] *= __builtin_amdgcn_rcpf(a.sight.cap);
 #pragma unroll
           for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[qt][tt][r] = quick_tanh(s[qt][tt][r] * by);
-          by = a.sight.cap * LOG2E;
+            for (int r = 0; r < 4; ++r) s[qt][tt][r] = quick_tanh(s[qt][tt][r] * by[qt]);
+          by[qt] = a.sight.cap * LOG2E;
         }
         if (masked) {
 #pragma unroll
@@ -1116,30 +1131,34 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt8_kernel(Attend a
               s[qt][tt][r] = key <= qpos[qt] && (key >= qlo[qt] || key < keep) ? s[qt][tt][r] : NEG_INF;
             }
         }
-        const float mn = fmaxf(run[qt].m, quad_rows_max(max_of_16(s[qt]) * by)), base = mn == NEG_INF ? 0.f : mn;
-        alpha[qt] = __builtin_amdgcn_exp2f(run[qt].m - base);
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        top[qt] = max_of_16(s[qt]) * by[qt];
+        grows = grows || top[qt] > run[qt].m + SLACK;
+      }
+      if (__any(grows)) {  // uniform; rare once the first keys have been seen
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+          const float mn = fmaxf(run[qt].m, quad_rows_max(top[qt]));
+          base[qt] = mn == NEG_INF ? 0.f : mn;
+          const float alpha = __builtin_amdgcn_exp2f(run[qt].m - base[qt]);
+          run[qt].m = mn;
+          l[qt] *= alpha;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) run[qt].o[d] *= alpha;
+        }
+      }
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float w = __builtin_amdgcn_exp2f(fmaf(s[qt][tt][r], by, -base));
-            sum[r] += w;
-            p[qt][tt >> 1][(tt & 1) * 4 + r] = (bf16)w;
-          }
-        run[qt].m = mn;
-        run[qt].l = run[qt].l * alpha[qt] + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-        rescale = rescale || alpha[qt] != 1.f;
-      }
-      if (__any(rescale)) {  // some query's maximum moved: rare once the first keys have been seen
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-          for (int d = 0; d < DT; ++d) run[qt].o[d] *= alpha[qt];
-      }
+          for (int r = 0; r < 4; ++r) p[qt][tt >> 1][(tt & 1) * 4 + r] = (bf16)__builtin_amdgcn_exp2f(fmaf(s[qt][tt][r], by[qt], -base[qt]));
       if constexpr (!EARLY) read_values(0);
       read_values(1);
       __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) l[qt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[qt][h], l[qt], 0, 0, 0);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -1153,17 +1172,16 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt8_kernel(Attend a
 
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
-    const float l = quad_rows_sum(run[qt].l);
     if (!working || qt * 16 + col >= nq) continue;
     const size_t row = (size_t)(tok0 + q0 + qt * 16 + col) * a.H + head;
     if (partial) {
       const size_t to = row * cut.pieces + it.piece;
-      if (grp == 0) *reinterpret_cast<float2*>(cut.ml + 2 * to) = make_float2(run[qt].m, l);
+      if (grp == 0) *reinterpret_cast<float2*>(cut.ml + 2 * to) = make_float2(run[qt].m, l[qt][0]);
 #pragma unroll
       for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4_t*>(cut.acc + to * D + 16 * d + 4 * grp) = run[qt].o[d];
       continue;
     }
-    const float inv = share_of(a.sight, head, run[qt].m, l);
+    const float inv = share_of(a.sight, head, run[qt].m, l[qt][0]);
 #pragma unroll
     for (int d = 0; d < DT; ++d) put4(a.out, row * D + 16 * d + 4 * grp, run[qt].o[d] * inv, a.sight.wide);
   }
