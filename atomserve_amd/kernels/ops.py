@@ -1057,14 +1057,14 @@ def attn_decode_fresh8(qkv, q_weight, k_weight, cos_sin, slots, eps, store_kv, k
          p_pos, p_tables, table_width, p_out, p_parts, H, KV, D, R, bs, float(scale), int(window), part_size, P, _stream())  # fmt: skip
 
 
-# What a step of portions over 8 bits costs, in microseconds fitted to the kernel's times of 435 steps (1 to 16 portions of 9 to 2,048 tokens behind 0 to
+# What a step of portions over 8 bits costs, in microseconds fitted to the kernel's times of 501 steps (1 to 16 portions of 9 to 2,048 tokens behind 0 to
 # 30,000; 16 to 64 heads of 64, 128, 192 and 256; 256 compute units), by (column tiles of 16 queries that a wave owns, head width): a round of 64 keys where a
 # workgroup has a compute unit to itself, a round where all places are taken, and the places.  Workgroups are counted as far as items are long enough to be
 # cut; items of every length (spread 1: a lone prompt) share their places less, and more workgroups than places last for all the work divided by the places and a
-# fifth of a piece, or whole turns as far as items are equally long.  What it picks takes 4 per cent more than the best of 16 forms on average and 54 at worst (the rule of
-# 16-bit pages, `_prefill_plan`, 8 and 106; for heads of 192, whose 32 queries a wave leave room for one workgroup, 6 and 32).
-PREFILL8_ROUNDS = {(1, 64): (0.70, 1.48, 4), (2, 64): (1.17, 2.07, 3), (1, 128): (0.89, 1.57, 3), (2, 128): (1.46, 2.09, 2), (1, 192): (1.45, 1.94, 2),
-                   (2, 192): (2.34, 2.76, 1), (1, 256): (1.65, 1.95, 1), (2, 256): (3.04, 3.42, 1)}  # fmt: skip
+# ninth of a piece, or as long as the longest piece, or whole turns as far as items are equally long.  What it picks takes 3 per cent more than the best of 16 forms on
+# average and 49 at worst (the rule of 16-bit pages, `_prefill_plan`, 8 and 95; for heads of 192, whose 32 queries a wave leave room for one workgroup, 3 and 29 on average).
+PREFILL8_ROUNDS = {(1, 64): (0.65, 1.35, 4), (2, 64): (1.01, 1.81, 3), (1, 128): (0.80, 1.46, 3), (2, 128): (1.28, 1.85, 2), (1, 192): (1.28, 1.80, 2),
+                   (2, 192): (2.13, 2.48, 1), (1, 256): (1.48, 1.77, 1), (2, 256): (2.65, 3.06, 1)}  # fmt: skip
 PREFILL8_PIECES = (1, 2, 3, 4, 6, 8, 12, 16)
 PREFILL8_MIN_PIECE_ROUNDS = 4
 
@@ -1081,9 +1081,9 @@ def _prefill8_cost(num_tiles, H, KV, D, rounds, mean_rounds, query_tiles, pieces
         cost = piece * (alone + (shared - alone) * (workgroups - units) / (places - units) * (1.0 - 0.55 * spread))
     else:
         work = num_tiles * KV * (64 // (16 * query_tiles)) * (H // KV) / 4 * mean_rounds  # rounds of full workgroups
-        evenly = max(piece * alone, (work / places + 0.2 * piece) * shared)
+        evenly = ((piece * alone) ** 4 + ((work / places + 0.11 * piece) * shared) ** 4) ** 0.25
         cost = spread * evenly + (1.0 - spread) * math.ceil(workgroups / places) * piece * shared
-    return cost + (6.7 + 64 * num_tiles * H * pieces * D * 8 / 9.7e6 if pieces > 1 else 0.0)
+    return cost + (6.7 + 64 * num_tiles * H * pieces * D * 8 / 9.0e6 if pieces > 1 else 0.0)
 
 
 @functools.lru_cache(maxsize=1024)
