@@ -462,10 +462,11 @@ template <int D> __device__ __forceinline__ f32x4_t score_tile(const u32x4_t (&k
   return s;
 }
 
-// What scores are taken relative to need not be their maximum: weights of up to 2^8 are as exact as those of up to 1.  So a maximum that has grown by less
-// moves nothing, and whether one has grown by more is all that a step asks; lanes agree on a new one, and sums are rescaled, only then.  (2,048 tokens behind
-// 14,336: 538 -> 493 us, ones in use as they were; wide heads and short portions alike.)
-constexpr float SLACK = 8.f;
+// What scores are taken relative to need not be their maximum: weights of up to 2 are as good as those of up to 1.  So a maximum that has grown by no more than a
+// factor of 2 moves nothing, and whether one has grown by more is all that a step asks; lanes agree on a new one, and sums are rescaled, only then.  2,048
+// tokens behind 14,336 take 458 us, 485 where every step does all of it, 472 where it does so for any growth and 445 where it does so for a growth beyond 2^8;
+// but a largest weight that is not 1 is rounded to bfloat16 itself: errors against 64 bits are 1.93e-3, 1.88e-3, 1.88e-3 and 2.12e-3.
+constexpr float SLACK = 1.f;  // in base 2
 
 template <int D> struct Running {
   f32x4_t o[D / 16];
@@ -906,11 +907,12 @@ __global__ __launch_bounds__(256) void single8_merge_kernel(Attend a, int D) {
 //
 // One barrier a round.  Where the blocks lie and their scales are looked up for 16 rounds at a time, a block a lane.
 //
-// Bound by what a SIMD issues: of a wave's round with QT 2 and heads of 128 the matrix cores are busy 1,026 cycles and the vector unit 1,283 (softmax, widening),
-// and the two waves of a SIMD take their sum, since a wave's products wait for its softmax.  2,048 tokens behind
-// 14,336 (32 heads on 8): 484 to 492 us, 1,050 TFLOP/s where an 8192^3 bf16 product reaches 1,212; 16-bit pages 522 to 537.  Keys read by every wave from memory, without LDS,
-// took 1,561.  A ring of four rounds in LDS was 3 to 20 per cent slower (room for fewer workgroups), a round's weighted values under the next
-// round's softmax 15 (spills), wave priorities no different.
+// Bound by the matrix cores' products and the softmax between them, at the clock that is left: with QT 2 and heads of 128 a wave's round is 52 products (1,090
+// cycles); matrix cores are busy 57 per cent of the time and the vector unit 49.  Sums of weights are products with ones, which the vector unit would take 128
+// cycles for (2 to 4 per cent of the time).  2,048 tokens behind 14,336 (32 heads on 8): 458 us, 1,125 TFLOP/s where an 8192^3
+// bf16 product reaches 1,212; 16-bit pages 535.  Keys read by every wave from memory, without LDS, took 1,561.  A ring of four rounds in LDS was
+// 3 to 20 per cent slower (room for fewer workgroups), a round's weighted values under the next round's softmax 15 (spills), widening between
+// the weighted values' products and wave priorities no different.
 //
 // A step of few work items takes as long as its longest one: with `pieces` > 1 an item comes as that many workgroups, an item of more than `piece_rounds`
 // rounds is cut along its keys, and what the pieces leave (maxima, sums, unnormalised outputs) is put together by a second kernel.
