@@ -940,7 +940,9 @@ def _partition8(N: int, H: int, KV: int, D: int, span: int, units: int, capped: 
 
 def _partitions8(N, H, KV, D, max_context, window, part_size, device, keep_first=0, capped=False):
     """`_partitions` for the kernel of single queries over 8 bits, whose steps are 64 keys."""
-    span = _up64(max_context) if window <= 0 else min(_up64(max_context), _up64(window + STEP8 - 1) + _up64(keep_first))
+    span = _up64(max(max_context, 1))  # a step whose queries see nothing asks for zeros all the same
+    if window > 0:
+        span = min(span, _up64(window + STEP8 - 1) + _up64(keep_first))
     if part_size is None:
         part_size = _partition8(N, H, KV, D, span, compute_units(), capped)
     if part_size <= 0 or part_size % STEP8:

@@ -256,6 +256,13 @@ def test_partitions_cover_what_is_seen(D, KV, group):
                 assert ops.contexts_cut8(N, H, KV, D, context, window, keep) == (P > 1)
 
 
+def test_a_step_whose_queries_see_nothing_is_a_step():
+    assert ops._partitions8(3, 32, 8, 128, 0, 0, None, "cuda:0") == (64, 1, None)
+    for call in (single, fresh, prompt):
+        with pytest.raises(AssertionError, match="would have been launched"):
+            call(max_context=0)
+
+
 def test_a_lone_long_context_is_cut_for_the_whole_gpu():
     part, P, _ = ops._partitions8(1, 32, 8, 128, 131_072, 0, None, "cuda:0")
     assert P * 8 >= 256 and part >= 256

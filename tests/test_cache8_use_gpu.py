@@ -246,3 +246,25 @@ def test_tensors_that_do_not_start_on_16_bytes_are_refused(ops):
     with pytest.raises(KernelError):
         ops.attn_decode_fresh8(odd(s.next_qkv), *s.gains, s.next_cos_sin, s.next_slots, 1e-6, True, *s.cache, s.next_positions, s.tables, s.next_out, s.H,
                                scale, 0, 601)  # fmt: skip
+
+
+@pytest.mark.parametrize("bs", [256, 1040])
+def test_large_pages(ops, bs):
+    from tests.test_cache8_gpu import prompt, single
+
+    single(ops, 8, 2, 128, bs, [1, 255, 256, 257, 1039, 1040, 1041, 1500])
+    single(ops, 7, 1, 64, bs, [2500, 3], part_size=128, window=1100)
+    prompt(ops, 4, 2, 128, bs, [(70, 0), (33, 1030), (100, 200)])
+
+
+def test_a_step_whose_queries_see_nothing(ops):
+    s = Step(ops)
+    none = torch.full((s.N,), -1, dtype=I32, device=DEV)
+    before = s.state()[3:]
+    for part in (None, 64):
+        out = torch.full((s.N, s.H, s.D), 7.0, dtype=BF16, device=DEV)
+        ops.attn_single_query8(s.q[: s.N], *s.cache, None, none, None, s.tables, out, 0.1, 0, 0, part_size=part)
+        assert not bool(out.any())
+        out.fill_(7.0)
+        ops.attn_decode_fresh8(s.next_qkv, *s.gains, s.next_cos_sin, none, 1e-6, True, *s.cache, none, s.tables, out, s.H, 0.1, 0, 0, part_size=part)
+        assert not bool(out.any()) and same(s.state()[3:], before)
