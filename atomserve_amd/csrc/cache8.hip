@@ -739,11 +739,19 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a
   const int h0 = kvh * G;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, grp = lane >> 4;
   const int t = a.items ? a.items[item] : item, bs = a.pages.nb * BLOCK;
+  const int* const table = a.tables + (size_t)(a.tok_row ? a.tok_row[t] : t) * a.table_width;
+  const int from = part * a.part_steps;
+  int at = from + wave;
+  // Where nothing hides the first keys, the entries of the first step are asked for beside the position: those beyond it, whatever they are, name
+  // numbers that the mask hides.
+  const bool whole = a.sight.window == 0 && a.sight.chunk == 0;
+  Blocks blocks{};
+  if (whole) blocks.ask(a.pages, Pieces{table, a.table_width * a.pages.nb - 1, a.magic}, STEP * min(at, (a.table_width * a.pages.nb - 1) / (STEP / BLOCK)));
   const int pos = min(a.positions[t], a.table_width * bs - 1);
   const int lo = first_in_window(a.sight, pos + 1);
-  const Pieces pieces{a.tables + (size_t)(a.tok_row ? a.tok_row[t] : t) * a.table_width, max(pos, 0) / BLOCK, a.magic};
+  const Pieces pieces{table, max(pos, 0) / BLOCK, a.magic};
   const Steps steps(lo, a.sight.keep, pos);
-  const int from = part * a.part_steps, to = min(steps.count, from + a.part_steps);
+  const int to = min(steps.count, from + a.part_steps);
   [[maybe_unused]] const int last = steps.count - 1;  // the step that ends with the token's own position
   [[maybe_unused]] const bool here = FRESH && fresh.store && last >= from && last < to;
   [[maybe_unused]] unsigned own_block = 0;
@@ -759,11 +767,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a
   }
   // a step's operands are asked for a step ahead, where they lie two steps ahead
   Held<D> even, odd;
-  Blocks blocks;
   const int page_head = kvh / a.share;
-  int at = from + wave;
   if (at < to) {
-    blocks.ask(a.pages, pieces, steps.first_key(at));
+    if (!whole) blocks.ask(a.pages, pieces, steps.first_key(at));
     load_step<D>(even, a.pages, blocks, page_head);
     if (at + 4 < to) blocks.ask(a.pages, pieces, steps.first_key(at + 4));
   }
