@@ -829,6 +829,21 @@ def _check8(t, name, dtype, shape, here: int) -> None:
         raise KernelError(f"{name} lies on cuda:{t.get_device()}, the current device is cuda:{here}")
 
 
+def _stream8(here: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(here)
+
+
+def _sight8(window, keep_first, chunk, softcap, sink, q, out, here: int) -> tuple:
+    """`_sight`, with results and sinks on the current device."""
+    if window == keep_first == chunk == softcap == 0 and sink is False and out.dtype is BF16:  # most calls
+        _check8(out, "out", BF16, q.shape, here)
+        return 0, 0, 0, 0.0, 0, 0, 0
+    sight = _sight(window, keep_first, chunk, softcap, sink, q, out)
+    if out.get_device() != here or (sight[5] and sink.get_device() != here):
+        raise KernelError(f"attention over 8 bits: results or sinks lie on another device than the current one, cuda:{here}")
+    return sight
+
+
 def _shape8(t, name, dims: int) -> tuple:
     """The shape of what has to be a tensor of `dims` dimensions."""
     if not isinstance(t, torch.Tensor) or t.dim() != dims:
@@ -902,7 +917,7 @@ def qk_norm_rope_store8(qkv, q_weight, k_weight, cos_sin, slots, q_out, k_pages,
         cache = slots, k_pages, v_pages, k_scales, v_scales
     p_qkv, p_qw, p_kw, p_cs, p_q, p_slots, *pages = _addresses(qkv, q_weight, k_weight, cos_sin if R else None, q_out, *cache)
     call("as_qk_norm_rope_store8", p_qkv, p_qw, p_kw, _DT[w_dtype], p_cs, p_slots, p_q, *pages, NB, T, num_heads, num_kv_heads, D, R, float(eps), bs,
-         int(bool(store_kv)), _stream())  # fmt: skip
+         int(bool(store_kv)), _stream8(here))  # fmt: skip
 
 
 def _up64(n: int) -> int:
@@ -971,9 +986,7 @@ def attn_single_query8(q, k_pages, v_pages, k_scales, v_scales, items, positions
     here = _device()
     T, H, D = shape = _shape8(q, "q", 3)
     _check8(q, "q", BF16, shape, here)
-    sight = _sight(window, keep_first, chunk, softcap, sink, q, out)
-    if out.get_device() != here or (sight[5] and sink.get_device() != here):
-        raise KernelError(f"attention over 8 bits: results or sinks lie on another device than the current one, cuda:{here}")
+    sight = _sight8(window, keep_first, chunk, softcap, sink, q, out, here)
     NB, KV, bs, width = _pages8(k_pages, v_pages, k_scales, v_scales, here)
     N = T
     if items is not None:
@@ -1001,7 +1014,7 @@ def attn_single_query8(q, k_pages, v_pages, k_scales, v_scales, items, positions
     p_q, p_k, p_v, p_ks, p_vs, p_items, p_pos, p_row, p_tables, p_out, p_parts = _addresses(
         q, k_pages, v_pages, k_scales, v_scales, items, positions, tok_row, block_tables, out, parts)
     call("as_attn_single_query8", p_q, p_k, p_v, p_ks, p_vs, NB, p_items, N, p_pos, p_row, p_tables, table_width, p_out, p_parts, H, KV * share, D, bs,
-         float(scale), *sight, part_size, P, share, _stream())  # fmt: skip
+         float(scale), *sight, part_size, P, share, _stream8(here))  # fmt: skip
 
 
 def attn_decode_fresh8_supported(dtype, num_heads: int, num_kv_heads: int, head_dim: int, block_size: int, rotary_dim: int) -> bool:
@@ -1056,7 +1069,7 @@ def attn_decode_fresh8(qkv, q_weight, k_weight, cos_sin, slots, eps, store_kv, k
         qkv, q_weight, k_weight, cos_sin if R else None, slots if store_kv else None, k_pages, v_pages, k_scales, v_scales, order, positions,
         block_tables, out, parts)  # fmt: skip
     call("as_attn_decode_fresh8", p_qkv, p_qw, p_kw, _DT[w_dtype], p_cs, p_slots, float(eps), int(bool(store_kv)), p_k, p_v, p_ks, p_vs, NB, p_order, T,
-         p_pos, p_tables, table_width, p_out, p_parts, H, KV, D, R, bs, float(scale), int(window), part_size, P, _stream())  # fmt: skip
+         p_pos, p_tables, table_width, p_out, p_parts, H, KV, D, R, bs, float(scale), int(window), part_size, P, _stream8(here))  # fmt: skip
 
 
 # What a step of portions over 8 bits costs, in microseconds fitted to the kernel's times of 501 steps (1 to 16 portions of 9 to 2,048 tokens behind 0 to
@@ -1108,9 +1121,7 @@ def attn_prefill8(q, k_pages, v_pages, k_scales, v_scales, tiles, block_tables, 
     here = _device()
     T, H, D = shape = _shape8(q, "q", 3)
     _check8(q, "q", BF16, shape, here)
-    sight = _sight(window, keep_first, chunk, softcap, sink, q, out)
-    if out.get_device() != here or (sight[5] and sink.get_device() != here):
-        raise KernelError(f"attention over 8 bits: results or sinks lie on another device than the current one, cuda:{here}")
+    sight = _sight8(window, keep_first, chunk, softcap, sink, q, out, here)
     NB, KV, bs, width = _pages8(k_pages, v_pages, k_scales, v_scales, here)
     num_tiles, _ = _shape8(tiles, "tiles", 2)
     _check8(tiles, "tiles", I32, (num_tiles, 4), here)
@@ -1131,7 +1142,7 @@ def attn_prefill8(q, k_pages, v_pages, k_scales, v_scales, tiles, block_tables, 
         parts = torch.empty(T * H * pieces * (D + 2) + num_tiles * KV * _prefill_units(query_tiles, H // KV), dtype=F32, device=q.device)
     p_q, p_k, p_v, p_ks, p_vs, p_tiles, p_tables, p_out, p_parts = _addresses(q, k_pages, v_pages, k_scales, v_scales, tiles, block_tables, out, parts)
     call("as_attn_prefill8", p_q, p_k, p_v, p_ks, p_vs, NB, p_tiles, num_tiles, p_tables, table_width, p_out, H, KV, D, bs, float(scale), *sight,
-         int(query_tiles), pieces, piece_rounds, p_parts, T, _stream())  # fmt: skip
+         int(query_tiles), pieces, piece_rounds, p_parts, T, _stream8(here))  # fmt: skip
 
 
 SKINNY_MAX_ROWS = 16  # up to here the bf16 product streams the weights through our own kernel

@@ -16,7 +16,7 @@ def nothing_is_launched(monkeypatch):
 
     monkeypatch.setattr(ops, "call", call)
     monkeypatch.setattr(ops, "_addresses", lambda *tensors: [0] * len(tensors))
-    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(ops, "_stream8", lambda here: 0)
     monkeypatch.setattr(ops, "_device", lambda: 0)
     monkeypatch.setattr(ops, "_compute_units", 256)
     with FakeTensorMode():  # tensors that say they are on the GPU, without memory
