@@ -89,8 +89,10 @@ def attend(q, k, v, position, scale, window=0, keep=0, chunk=0, cap=0.0, sink=No
     total = w.sum(-1, keepdim=True) + (torch.exp(sink.to(F64)[:, None] - top) if sink is not None else 0.0)
     out = (w[:, None] @ v)[:, 0] / total
     size = (w[:, None] @ v.abs())[:, 0] / total
-    # weights rounded to bfloat16 (2^-8 of each), the result once more, scores' errors in numerator and denominator, sums in 32 bits
-    return out, 2.0**-8 * (size + out.abs()) + (2 * off + 2.0**-16) * size + 1e-30
+    # Weights rounded to bfloat16, w (1 + e) with |e| <= 2^-8: with the sum of those that are not rounded as the denominator the result is off by
+    # |sum w e v| / sum w <= 2^-8 size; with the sum of the rounded ones by |sum w e (v - out)| / sum w (1 + e), which is at most
+    # 2^-8 (size + |out|) (1 + 2^-7).  The result is rounded once more, 2^-8 |out|.  Scores' errors count in numerator and denominator, sums are 32-bit.
+    return out, 2.0**-8 * (1 + 2.0**-7) * (size + 2 * out.abs()) + (2 * off + 2.0**-16) * size + 1e-30
 
 
 def gathered(cache, table, length):
