@@ -64,7 +64,7 @@ __device__ __forceinline__ size_t block_index(const Pages& p, int page, int kvh,
 // block, so that a coordinate's bytes are neighbours in a lane's hands: they cross to the transposed block through LDS.
 //
 // Bound by memory where there is much of it (a prompt of 2,048 tokens, 32 heads of 128 on 8: 11.4 us, 47 MB at 4.2 TB/s; 16-bit pages 12.7) and by a launch
-// and three dependent waits (slots, scale, stores) where there is not: one token 3.0 us, 64 requests' tokens 4.6, 2.6 of it the queries.
+// and three dependent waits (slots, scale, stores) where there is not: one token 3.0 us, 64 requests' tokens 4.0, 2.6 of it the queries.
 template <int D> struct Lanes {
   static constexpr int LPT = D <= 64 ? 8 : D <= 128 ? 16 : 32;  // lanes of a head, D / 8 of them busy
   static constexpr int AT_ONCE = WAVE / LPT, PASSES = BLOCK / AT_ONCE;
@@ -280,6 +280,7 @@ __device__ __forceinline__ void append_run(const Append& a, int t, int n, int sl
 
 // Single tokens (decode steps), as many as a wave has groups of lanes, each group one: `tokens` has the lanes that look at them, `slot` what lane l looks at.
 // Nothing crosses lanes: a key is a row, a value a byte of every coordinate's 16, and only a scale that grows makes the rest of the block be read.
+// Lane j has every (D / 8)th coordinate of a value, from j on: neighbours' bytes are 16 apart, and a store is a few lines of memory instead of one a lane.
 template <int D, typename W, bool VALUES>
 __device__ __forceinline__ void append_singles(const Append& a, int t0, unsigned long long& tokens, int slot, int kvh, const float (&g)[8]) {
   constexpr int LPT = Lanes<D>::LPT, AT_ONCE = Lanes<D>::AT_ONCE;
@@ -307,8 +308,13 @@ __device__ __forceinline__ void append_singles(const Append& a, int t0, unsigned
   const bf16* src = a.qkv + ((size_t)t * heads + a.H + (VALUES ? a.pages.KV : 0) + kvh) * D;
   const float before = off > 0 ? scales[block] : 0.f;  // a block that begins with this token is new
   float x[8];
-  load4(src + at.a, x);
-  load4(src + at.b, x + 4);
+  if constexpr (VALUES) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)src[D / 8 * i + (busy ? j : 0)];
+  } else {
+    load4(src + at.a, x);
+    load4(src + at.b, x + 4);
+  }
   if constexpr (!VALUES) norm_turn<D>(x, a.kw != nullptr, g, a.cs, a.eps, R, t, j, busy);
   float amax = 0.f;
 #pragma unroll
@@ -334,7 +340,7 @@ __device__ __forceinline__ void append_singles(const Append& a, int t0, unsigned
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const unsigned byte = (i < 4 ? lower : upper) >> (8 * (i & 3)) & 0xffu;
-      uint8_t* piece = base + (8 * j + i) * BLOCK;
+      uint8_t* piece = base + (D / 8 * i + j) * BLOCK;
       if (grows) {
         u32x4_t held = *reinterpret_cast<const u32x4_t*>(piece);
 #pragma unroll
@@ -1293,10 +1299,11 @@ extern "C" int as_qk_norm_rope_store8(const void* qkv, const void* qw, const voi
   if (store && (!slots || !pages_ok(k_pages, v_pages, k_scales, v_scales, num_pages, KV, D, bs))) return AS_BAD_SHAPE;
   if (w_dtype != DT_F32 && w_dtype != DT_BF16) return AS_BAD_DTYPE;
   if (R == 0) cs = nullptr;
-  // Tokens whose runs a wave takes: 16 is a block, so that a prompt's waves have one run each; with few (token, kv head) pairs compute units would stay
-  // empty.  us with 4 / with 16, 32 heads of 128 on 8: single tokens of 64 requests 4.7 / 9.2, of 256 6.4 / 11.1; prompts of 512 5.5 / 5.0, of 2,048
-  // 17.5 / 11.9, of 8,192 61.7 / 38.6.
-  const int chunk = (long long)num_tokens * KV <= 2048 ? 4 : 16;
+  // Tokens whose runs a wave takes: 16 is a block, so that a prompt's waves have one run each, but single tokens, four at a time, are a chain of up to four
+  // turns then.  us with 4 / 8 / 16, 32 heads of 128 on 8: single tokens of 64 requests 4.0 / 4.9 / 6.8, of 256 4.8 / 5.7 / 7.4, of 512 6.7 / 6.5 / 8.1; prompts
+  // of 512 5.4 / 5.0 / 4.9, of 2,048 17.5 / 14.0 / 11.8, of 480 beside 32 single tokens 5.5 / 5.2 / 7.0.
+  const long long pairs = (long long)num_tokens * KV;
+  const int chunk = pairs <= 2048 ? 4 : pairs <= 6144 ? 8 : 16;
   const long long kv_blocks = store ? (((long long)num_tokens + chunk - 1) / chunk * 2 * KV + 3) / 4 : 0;
   const Append a{(const bf16*)qkv, qw, kw, (const float2*)cs, slots, (bf16*)q_out, pages_of(k_pages, v_pages, k_scales, v_scales, num_pages, KV, bs),
            num_tokens, H, R, eps, chunk, (int)kv_blocks};
