@@ -419,6 +419,16 @@ template <int D> struct Query {
   float scale;
 };
 
+// Four numbers of a query, scaled, as their two parts.
+__device__ __forceinline__ void split4(const float* x, float inv, unsigned& high, unsigned& low) {
+  float y[4];
+#pragma unroll
+  for (int n = 0; n < 4; ++n) y[n] = at_most_largest(x[n] * inv);
+  high = pack4(y[0], y[1], y[2], y[3]);
+  const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)high, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)high, true);
+  low = pack4(y[0] - a[0], y[1] - a[1], y[2] - b[0], y[3] - b[1]);
+}
+
 template <int D> __device__ __forceinline__ void load_query(Query<D>& q, const bf16* row, int grp) {
   float x[D / 64][16];
   unsigned most = 0;  // the largest magnitude's bits: of a query that is not finite those of an infinity or more
@@ -437,13 +447,10 @@ template <int D> __device__ __forceinline__ void load_query(Query<D>& q, const b
   for (int c = 0; c < D / 64; ++c)
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      float y[4];
-#pragma unroll
-      for (int n = 0; n < 4; ++n) y[n] = at_most_largest(x[c][4 * w + n] * inv);
-      const unsigned high = pack4(y[0], y[1], y[2], y[3]);
-      const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)high, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)high, true);
+      unsigned high, low;
+      split4(x[c] + 4 * w, inv, high, low);
       q.high[c][w] = high;
-      q.low[c][w] = pack4(y[0] - a[0], y[1] - a[1], y[2] - b[0], y[3] - b[1]);
+      q.low[c][w] = low;
     }
   if (amax == __builtin_inff()) q.scale = __builtin_nanf("");  // no e4m3 number stands for it: what it sees becomes NaN, and none of its neighbours
 }
@@ -668,6 +675,13 @@ struct Fresh {
   int store;    // 0: queries only, the block already holds the token
 };
 
+// A query as the lanes that normed it leave it in LDS: the parts that `load_query` makes.
+template <int D> struct Split {
+  unsigned high[D / 4], low[D / 4];
+  float scale;
+  unsigned apart[3];
+};
+
 // The token's key and value as its block holds them, in LDS.
 template <int D> struct News {
   unsigned bytes[2][D / 4];
@@ -675,44 +689,69 @@ template <int D> struct News {
   float by[2];     // what the block's other numbers are multiplied by: below 1 where the scale grows
 };
 
-// They go into the operands of the step that holds the token, its place in the step being `nth`, and with `write` into the block.
+// They go into the operands of the step that holds the token, its place in the step being `nth`, and with `write` into the block.  All that LDS holds is read at
+// once and chosen from without branches: reading where it was needed, this took 1.4 us of a wave that everybody waits for.
 template <int D>
 __device__ __forceinline__ void insert(Held<D>& held, const News<D>& news, int nth, const Pages& pages, unsigned block, bool write) {
   const int lane = threadIdx.x & (WAVE - 1), col = lane & 15, grp = lane >> 4, piece = nth >> 4, off = nth & 15;
-  const float kby = news.by[0], vby = news.by[1];
-  if (col >> 2 == piece) {  // this lane's keys are the block's
-    uint8_t* const rows = pages.k + (size_t)block * (BLOCK * D) + 16 * grp;
+  u32x4_t key[D / 64];
+  unsigned value[D / 16];
 #pragma unroll
-    for (int tt = 0; tt < 4; ++tt) {
-      const int row = 4 * tt + (col & 3);
+  for (int c = 0; c < D / 64; ++c) key[c] = *reinterpret_cast<const u32x4_t*>(&news.bytes[0][16 * c + 4 * grp]);
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d) value[d] = news.bytes[1][4 * d + (col >> 2)];
+  const float kby = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(news.by[0])));
+  const float vby = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(news.by[1])));
+  const float ks = news.scale[0], vs = news.scale[1];
+  const bool my_keys = col >> 2 == piece, my_values = grp == piece;  // this lane's are the block's
+  uint8_t* const rows = pages.k + (size_t)block * (BLOCK * D) + 16 * grp;
+  if (kby < 1.f && my_keys) {
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) {
-        if (kby < 1.f)  // uniform
 #pragma unroll
-          for (int w = 0; w < 4; ++w) held.k[tt][c][w] = rescale4(held.k[tt][c][w], kby);
-        if (row == off) held.k[tt][c] = *reinterpret_cast<const u32x4_t*>(&news.bytes[0][16 * c + 4 * grp]);
-        if (write && (kby < 1.f || row == off)) *reinterpret_cast<u32x4_t*>(rows + row * D + 64 * c) = held.k[tt][c];
+        for (int w = 0; w < 4; ++w) held.k[tt][c][w] = rescale4(held.k[tt][c][w], kby);
+        if (write) *reinterpret_cast<u32x4_t*>(rows + (4 * tt + (col & 3)) * D + 64 * c) = held.k[tt][c];
       }
-    }
   }
-  if (grp == piece) {
-    held.ks = news.scale[0];
-    held.vs = news.scale[1];
-    const unsigned shift = 8 * (off & 3), byte = 0xffu << shift;
-    u32x4_t* const vcol = reinterpret_cast<u32x4_t*>(pages.v + (size_t)block * (BLOCK * D)) + col;
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) {
-      const unsigned fresh = (news.bytes[1][4 * d + (col >> 2)] >> (8 * (col & 3)) & 0xffu) << shift;
+  for (int tt = 0; tt < 4; ++tt) {
+    const bool hit = my_keys && 4 * tt + (col & 3) == off;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        if (vby < 1.f) held.v[d][w] = rescale4(held.v[d][w], vby);
-        if (off >> 2 == w) held.v[d][w] = (held.v[d][w] & ~byte) | fresh;
-      }
-      if (write) vcol[16 * d] = held.v[d];
-    }
-    if (write && col == 0) {
-      pages.ks[block] = held.ks;
-      pages.vs[block] = held.vs;
+    for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) held.k[tt][c][w] = hit ? key[c][w] : held.k[tt][c][w];
+  }
+  if (write && my_keys && (col & 3) == (off & 3)) {
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) *reinterpret_cast<u32x4_t*>(rows + off * D + 64 * c) = key[c];
+  }
+  if (vby < 1.f && my_values) {
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) held.v[d][w] = rescale4(held.v[d][w], vby);
+  }
+  const unsigned byte = my_values ? 0xffu << (8 * (off & 3)) : 0u;
+  unsigned mine[4];  // where the value's byte lies in a coordinate's 16
+#pragma unroll
+  for (int w = 0; w < 4; ++w) mine[w] = off >> 2 == w ? byte : 0u;
+  u32x4_t* const vcol = reinterpret_cast<u32x4_t*>(pages.v + (size_t)block * (BLOCK * D)) + col;
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d) {
+    const unsigned fresh = (value[d] >> (8 * (col & 3)) & 0xffu) << (8 * (off & 3));
+#pragma unroll
+    for (int w = 0; w < 4; ++w) held.v[d][w] = (held.v[d][w] & ~mine[w]) | (fresh & mine[w]);
+  }
+  held.ks = my_values ? ks : held.ks;
+  held.vs = my_values ? vs : held.vs;
+  if (write && my_values) {
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) vcol[16 * d] = held.v[d];
+    if (col == 0) {
+      pages.ks[block] = ks;
+      pages.vs[block] = vs;
     }
   }
 }
@@ -729,7 +768,7 @@ __device__ __forceinline__ void insert(Held<D>& held, const News<D>& news, int n
 template <int D, bool FRESH, typename W>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a, Fresh fresh) {
   constexpr int LD = D + 4;
-  extern __shared__ __align__(16) float smem[];  // [4][16] m, [4][16] l, [4][G][LD]; FRESH: the news, [G][D + 8] bf16 queries
+  extern __shared__ __align__(16) float smem[];  // [4][16] m, [4][16] l, [4][G][LD]; FRESH: the news, [G] queries
   const int G = a.H / a.KV, part = blockIdx.y, N = gridDim.x / a.KV;
   int item = blockIdx.x / a.KV, kvh = blockIdx.x - item * a.KV;
   if (a.P == 1) {
@@ -786,7 +825,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a
   if constexpr (FRESH) {
     constexpr int LPT = Lanes<D>::LPT, AT_ONCE = Lanes<D>::AT_ONCE;
     const Append& f = fresh.from;
-    bf16* const queries = reinterpret_cast<bf16*>(news + 1);
+    Split<D>* const queries = reinterpret_cast<Split<D>*>(news + 1);
     const int j = lane % LPT, jobs = G + (here ? 2 : 0), heads = a.H + 2 * a.KV;
     const bool busy = 8 * j < D;
     for (int job = wave * AT_ONCE + lane / LPT; job < jobs; job += 4 * AT_ONCE) {  // the group's queries, the key, the value; whole lane groups
@@ -804,10 +843,18 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a
       }
       if (job <= G) norm_turn<D>(x, gains != nullptr, g, f.cs, f.eps, f.R, t, j, busy);
       if (query) {
+        unsigned most = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[i] = (float)(bf16)x[i];
+          most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
+        }
+        const float amax = lanes_max<LPT>(busy ? __uint_as_float(min(most, 0x7f800000u)) : 0.f), scale = block_scale(amax), inv = inverse_of(scale);
         if (!busy) continue;
-        bf16* to8 = queries + job * (D + 8);
-        *reinterpret_cast<bf16x4_t*>(to8 + at8.a) = bf16x4_t{(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]};
-        *reinterpret_cast<bf16x4_t*>(to8 + at8.b) = bf16x4_t{(bf16)x[4], (bf16)x[5], (bf16)x[6], (bf16)x[7]};
+        Split<D>& to8 = queries[job];
+        split4(x, inv, to8.high[at8.a / 4], to8.low[at8.a / 4]);
+        split4(x + 4, inv, to8.high[at8.b / 4], to8.low[at8.b / 4]);
+        if (j == 0) to8.scale = amax == __builtin_inff() ? __builtin_nanf("") : scale;
       } else {
         float amax = 0.f;
 #pragma unroll
@@ -828,7 +875,13 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a
       }
     }
     __syncthreads();
-    load_query<D>(q, queries + min(col, G - 1) * (D + 8), grp);
+    const Split<D>& from8 = queries[min(col, G - 1)];
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+      q.high[c] = *reinterpret_cast<const u32x4_t*>(&from8.high[16 * c + 4 * grp]);
+      q.low[c] = *reinterpret_cast<const u32x4_t*>(&from8.low[16 * c + 4 * grp]);
+    }
+    q.scale = from8.scale;
   } else {
     load_query<D>(q, a.q + ((size_t)t * a.H + h0 + min(col, G - 1)) * D, grp);
   }
@@ -857,22 +910,28 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f32x4_t*>(so + (wave * G + col) * LD + d * 16 + 4 * grp) = run.o[d];
   __syncthreads();
-  for (int i = tid; i < G * D; i += 256) {
-    const int g = i / D, d = i % D, h = h0 + g;
-    float m = NEG_INF, num = 0.f, den = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) m = fmaxf(m, sm[w * 16 + g]);
+  for (int i = tid; i < G * D / 4; i += 256) {  // four coordinates a thread
+    const int g = i / (D / 4), d = i % (D / 4) * 4, h = h0 + g;
+    float m = NEG_INF, den = 0.f, ms[4], ls[4];
+    f32x4_t num = {0.f, 0.f, 0.f, 0.f}, acc[4];
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float e = m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(sm[w * 16 + g] - m);
-      num += so[(w * G + g) * LD + d] * e;
-      den += sl[w * 16 + g] * e;
+      ms[w] = sm[w * 16 + g];
+      ls[w] = sl[w * 16 + g];
+      acc[w] = *reinterpret_cast<const f32x4_t*>(so + (w * G + g) * LD + d);
+      m = fmaxf(m, ms[w]);
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float e = m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(ms[w] - m);
+      num += acc[w] * e;
+      den += ls[w] * e;
     }
     if (a.P == 1) {
-      put(a.out, ((size_t)t * a.H + h) * D + d, num * share_of(a.sight, h, m, den), a.sight.wide);
+      put4(a.out, ((size_t)t * a.H + h) * D + d, num * share_of(a.sight, h, m, den), a.sight.wide);
     } else {
       const size_t o = ((size_t)item * a.H + h) * a.P + part;
-      a.part_acc[o * D + d] = num;
+      *reinterpret_cast<f32x4_t*>(a.part_acc + o * D + d) = num;
       if (d == 0) { a.part_m[o] = m; a.part_l[o] = den; }
     }
   }
@@ -1374,7 +1433,7 @@ extern "C" int as_attn_decode_fresh8(const void* qkv, const void* qw, const void
   const Attend a{nullptr, pages, items, positions, nullptr, nullptr, block_tables, table_width, (bf16*)out, parts + rows * D, parts + rows * (D + 1),
                  parts, H, KV, 1, scale, sight, part_size / STEP, P, magic_of(bs), compute_units()};
   const Fresh fresh{Append{(const bf16*)qkv, qw, kw, (const float2*)cs, slots, nullptr, pages, num_tokens, H, R, eps, 0, 0}, store};
-  const size_t shmem = sizeof(float) * (128 + 4 * (size_t)(D + 4) * (H / KV) + 4) + 2 * (size_t)D + sizeof(bf16) * (size_t)(D + 8) * (H / KV);
+  const size_t shmem = sizeof(float) * (128 + 4 * (size_t)(D + 4) * (H / KV) + 4) + 2 * (size_t)D + (2 * (size_t)D + 16) * (H / KV);
 #define LAUNCH2(DV, W)                                                                                                                   \
   {                                                                                                                                      \
     const auto kernel = single8_kernel<DV, true, W>;                                                                                     \
