@@ -14,6 +14,8 @@
 #include "attn_parts.h"
 #include "wide_tile.h"
 
+#include <algorithm>
+
 namespace {
 
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
@@ -636,6 +638,13 @@ __device__ __forceinline__ void put4(bf16* out, size_t i, f32x4_t v, int wide) {
   else *reinterpret_cast<bf16x4_t*>(out + i) = bf16x4_t{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
 }
 
+// Division by a number that a whole grid divides by, as a product: exact while dividend times divisor stays under 2^32.
+struct Divide {
+  unsigned by, magic;
+  explicit Divide(unsigned by) : by(by), magic(by > 1 ? (unsigned)((0x100000000ull + by - 1) / by) : 0u) {}
+  __device__ __forceinline__ int operator()(unsigned n) const { return by == 1 ? n : __umulhi(n, magic); }
+};
+
 struct Attend {
   const bf16* q;
   Pages pages;
@@ -653,6 +662,7 @@ struct Attend {
   int part_steps, P;
   unsigned magic;  // of a page's blocks (`Pieces`)
   int cus;
+  Divide kv, group;  // by KV and H / KV
 };
 
 __device__ __forceinline__ float score_factor(const Attend& a) { return a.sight.cap > 0.f ? a.scale : a.scale * LOG2E; }
@@ -769,13 +779,13 @@ template <int D, bool FRESH, typename W>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a, Fresh fresh) {
   constexpr int LD = D + 4;
   extern __shared__ __align__(16) float smem[];  // [4][16] m, [4][16] l, [4][G][LD]; FRESH: the news, [G] queries
-  const int G = a.H / a.KV, part = blockIdx.y, N = gridDim.x / a.KV;
-  int item = blockIdx.x / a.KV, kvh = blockIdx.x - item * a.KV;
-  if (a.P == 1) {
+  const int G = a.group.by, part = blockIdx.y;
+  int item = a.kv(blockIdx.x), kvh = blockIdx.x - item * a.KV;
+  if (a.P == 1 && (int)gridDim.x > a.cus) {
     // Whole contexts of unequal length, a workgroup each, two of them on a compute unit.  Taken eight items at a time, their kv heads one after the
     // other, with the second round of workgroups backwards: with `items` sorted longest first a compute unit's first two are a long and a short one.
     int s = blockIdx.x;
-    const int total = N * a.KV;
+    const int total = gridDim.x, N = a.kv(total);
     if (s >= a.cus && s < 2 * a.cus) s = a.cus + (min(2 * a.cus, total) - 1 - s);
     const int first = s / (8 * a.KV) * 8, r = s % (8 * a.KV), here = min(8, N - first);
     item = first + r % here;
@@ -812,7 +822,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a
   }
   // a step's operands are asked for a step ahead, where they lie two steps ahead
   Held<D> even, odd;
-  const int page_head = kvh / a.share;
+  const int page_head = a.share > 1 ? kvh / a.share : kvh;
   if (at < to) {
     if (!whole) blocks.ask(a.pages, pieces, steps.first_key(at));
     load_step<D>(even, a.pages, blocks, page_head);
@@ -1001,29 +1011,34 @@ template <int D> __device__ __forceinline__ int swizzle(int key) {  // of a key 
 
 struct Item {  // what a workgroup and a wave of it work on
   int item, tile, kvh, bz, piece;
-  __device__ __forceinline__ Item(const Attend& a, int units_z, int pass, int pieces) {
+  __device__ __forceinline__ Item(const Attend& a, const Divide& units_z, const Divide& pass, const Divide& pieces) {
     // Items in the order of `tiles`, those that see most keys first; runs of `pass` of them alternate direction, so that a compute unit that
     // received one of the longest in one round of workgroups receives one of the shortest in the next.
     int n = blockIdx.x;
-    const int block = n / pass, first = block * pass, size = min(pass, (int)gridDim.x - first), per_tile = a.KV * units_z;
+    const int block = pass(n), first = block * pass.by, size = min((int)pass.by, (int)gridDim.x - first);
     if (block & 1) n = first + size - 1 - (n - first);
-    piece = n % pieces;
-    item = n / pieces;
-    tile = item / per_tile;
-    kvh = item % per_tile / units_z;
-    bz = item % units_z;
+    item = pieces(n);
+    piece = n - item * pieces.by;
+    split(a, units_z);
+  }
+  __device__ __forceinline__ Item(const Attend& a, const Divide& units_z, int item) : item(item) { split(a, units_z); }
+  __device__ __forceinline__ void split(const Attend& a, const Divide& units_z) {
+    const int heads = units_z(item);
+    bz = item - heads * units_z.by;
+    tile = a.kv(heads);
+    kvh = heads - tile * a.KV;
   }
 };
 
 template <int D, int QT>
-__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt8_kernel(Attend a, int units_z, int pass, Cut cut) {
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt8_kernel(Attend a, Divide units_z, Divide pass, Divide pieces, Cut cut) {
   constexpr int DT = D / 16, WQ = 16 * QT, PARTS = 64 / WQ;  // queries of a wave; waves that share a head's 64 queries
   constexpr int KEYS = STEP * D, VALUES = 2 * STEP * D;      // bytes of a round
   __shared__ __align__(128) char keys[2][KEYS];
   __shared__ __align__(128) char values[2][VALUES];
-  const Item it(a, units_z, pass, cut.pieces);
+  const Item it(a, units_z, pass, pieces);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, grp = lane >> 4;
-  const int G = a.H / a.KV, kvh = it.kvh, end = a.table_width * a.pages.nb * BLOCK - 1;
+  const int G = a.group.by, kvh = it.kvh, end = a.table_width * a.pages.nb * BLOCK - 1;
   const int tok0 = a.tiles[4 * it.tile], count = a.tiles[4 * it.tile + 1], pos0 = max(a.tiles[4 * it.tile + 3], 0);
   const int* const table = a.tables + (size_t)a.tiles[4 * it.tile + 2] * a.table_width;
   auto first_seen = [&](int pos) { return first_in_window(a.sight, pos + 1); };
@@ -1031,7 +1046,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt8_kernel(Attend a
   // the keys this workgroup walks: from the first key that any of its waves sees to the last
   int wg_lo = 0x7fffffff, wg_last = -1;
   for (int u = it.bz * 4; u < it.bz * 4 + 4 && u < PARTS * G; ++u) {
-    const int uq0 = u / G * WQ;
+    const int uq0 = a.group(u) * WQ;
     if (uq0 >= count) continue;
     wg_last = max(wg_last, min(pos0 + min(count, uq0 + WQ) - 1, end));
     wg_lo = min(wg_lo, first_seen(min(pos0 + uq0, end)));
@@ -1057,7 +1072,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt8_kernel(Attend a
   const int rounds = rd_end - rd_first;
 
   // this wave's queries
-  const int unit = it.bz * 4 + wave, head = kvh * G + unit % G, q0 = unit / G * WQ;
+  const int unit = it.bz * 4 + wave, part = a.group(unit), head = kvh * G + unit - part * G, q0 = part * WQ;
   const bool working = unit < PARTS * G && q0 < count;
   const int nq = working ? min(WQ, count - q0) : 1;
   const int my_first = min(pos0 + q0, end), my_last = working ? min(pos0 + q0 + nq - 1, end) : -1;
@@ -1300,14 +1315,15 @@ __device__ __forceinline__ void merge_row(const Attend& a, const Cut& cut, size_
 }
 
 template <int D, int QT>
-__global__ __launch_bounds__(256) void prompt8_merge_kernel(Attend a, int units_z, Cut cut) {
+__global__ __launch_bounds__(256) void prompt8_merge_kernel(Attend a, Divide units_z, Cut cut) {
   constexpr int WQ = 16 * QT, PARTS = 64 / WQ;
   const int item = blockIdx.x, n = cut.cut[item];
   if (n <= 1) return;
-  const int G = a.H / a.KV, per_tile = a.KV * units_z, tile = item / per_tile, kvh = item % per_tile / units_z, bz = item % units_z;
+  const Item it(a, units_z, item);
+  const int G = a.group.by, tile = it.tile;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, at = 32 * blockIdx.y + 4 * (lane >> 4);
   const int tok0 = a.tiles[4 * tile], count = a.tiles[4 * tile + 1];
-  const int unit = bz * 4 + wave, head = kvh * G + unit % G, q0 = unit / G * WQ;
+  const int unit = it.bz * 4 + wave, part = a.group(unit), head = it.kvh * G + unit - part * G, q0 = part * WQ;
   if (unit >= PARTS * G || q0 >= count) return;
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
@@ -1390,13 +1406,13 @@ extern "C" int as_attn_single_query8(const void* q, const void* k_pages, const v
   const Sight sight{window, keep, chunk, cap, sink, sinks, wide};
   if (!sight_ok(sight) || H <= 0 || KV <= 0 || H % KV || H / KV > 16 || share < 1 || KV % share) return AS_BAD_SHAPE;
   if (!pages_ok(k_pages, v_pages, k_scales, v_scales, num_pages, KV / share, D, bs) || !table_ok(num_pages, KV / share, bs, table_width)) return AS_BAD_SHAPE;
-  if (!q || !positions || !block_tables || !out || !on_16_bytes(q, out, parts) || part_size <= 0 || part_size % STEP || P <= 0 || P > 65535 || (long long)num_items * KV > 0x7fffffffll)
+  if (!q || !positions || !block_tables || !out || !on_16_bytes(q, out, parts) || part_size <= 0 || part_size % STEP || P <= 0 || P > 65535 || (long long)num_items * KV * KV > 0xffffffffll)
     return AS_BAD_SHAPE;
   if (P > 1 && !parts) return AS_BAD_SHAPE;
   const size_t rows = P > 1 ? (size_t)num_items * H * P : 0;
   const Attend a{(const bf16*)q, pages_of(k_pages, v_pages, k_scales, v_scales, num_pages, KV / share, bs), items, positions, tok_row, nullptr,
                  block_tables, table_width, (bf16*)out, parts + rows * D, parts + rows * (D + 1), parts, H, KV, share, scale, sight, part_size / STEP, P,
-                 magic_of(bs), compute_units()};
+                 magic_of(bs), compute_units(), Divide(KV), Divide(H / KV)};
   const size_t shmem = sizeof(float) * (128 + 4 * (size_t)(D + 4) * (H / KV));
 #define LAUNCH(DV)                                                                                                                       \
   {                                                                                                                                      \
@@ -1425,13 +1441,13 @@ extern "C" int as_attn_decode_fresh8(const void* qkv, const void* qw, const void
   if (!pages_ok(k_pages, v_pages, k_scales, v_scales, num_pages, KV, D, bs) || !table_ok(num_pages, KV, bs, table_width)) return AS_BAD_SHAPE;
   if (!qkv || (qw == nullptr) != (kw == nullptr) || (store && !slots) || !positions || !block_tables || !out || !on_16_bytes(qkv, qw, kw, cs, out, parts))
     return AS_BAD_SHAPE;
-  if (part_size <= 0 || part_size % STEP || P <= 0 || P > 65535 || (long long)num_tokens * KV > 0x7fffffffll) return AS_BAD_SHAPE;
+  if (part_size <= 0 || part_size % STEP || P <= 0 || P > 65535 || (long long)num_tokens * KV * KV > 0xffffffffll) return AS_BAD_SHAPE;
   if (P > 1 && !parts) return AS_BAD_SHAPE;
   if (w_dtype != DT_F32 && w_dtype != DT_BF16) return AS_BAD_DTYPE;
   const size_t rows = P > 1 ? (size_t)num_tokens * H * P : 0;
   const Pages pages = pages_of(k_pages, v_pages, k_scales, v_scales, num_pages, KV, bs);
   const Attend a{nullptr, pages, items, positions, nullptr, nullptr, block_tables, table_width, (bf16*)out, parts + rows * D, parts + rows * (D + 1),
-                 parts, H, KV, 1, scale, sight, part_size / STEP, P, magic_of(bs), compute_units()};
+                 parts, H, KV, 1, scale, sight, part_size / STEP, P, magic_of(bs), compute_units(), Divide(KV), Divide(H / KV)};
   const Fresh fresh{Append{(const bf16*)qkv, qw, kw, (const float2*)cs, slots, nullptr, pages, num_tokens, H, R, eps, 0, 0}, store};
   const size_t shmem = sizeof(float) * (128 + 4 * (size_t)(D + 4) * (H / KV) + 4) + 2 * (size_t)D + (2 * (size_t)D + 16) * (H / KV);
 #define LAUNCH2(DV, W)                                                                                                                   \
@@ -1472,15 +1488,16 @@ extern "C" int as_attn_prefill8(const void* q, const void* k_pages, const void* 
   if (pieces > 1 && (piece_rounds < 1 || !parts || tokens <= 0)) return AS_BAD_SHAPE;
   const int units_z = (64 / (16 * query_tiles) * (H / KV) + 3) / 4;
   const long long items = (long long)num_tiles * KV * units_z;
-  if (items * pieces > 0x7fffffffll) return AS_BAD_SHAPE;
+  if (items * pieces > 0xffffffffll / std::max(std::max(pieces, compute_units()), std::max(units_z, KV))) return AS_BAD_SHAPE;  // `Divide`
+  const Divide z(units_z), pass(compute_units()), by_pieces(pieces);
   const Attend a{(const bf16*)q, pages_of(k_pages, v_pages, k_scales, v_scales, num_pages, KV, bs), nullptr, nullptr, nullptr, tiles, block_tables,
-                 table_width, (bf16*)out, nullptr, nullptr, nullptr, H, KV, 1, scale, sight, 0, 1, magic_of(bs), compute_units()};
+                 table_width, (bf16*)out, nullptr, nullptr, nullptr, H, KV, 1, scale, sight, 0, 1, magic_of(bs), compute_units(), Divide(KV), Divide(H / KV)};
   const size_t rows = pieces > 1 ? (size_t)tokens * H * pieces : 0;
   const Cut how{pieces, piece_rounds, (int*)(parts + rows * (D + 2)), parts + rows * D, parts};
 #define LAUNCH2(DV, QTV)                                                                                           \
   {                                                                                                                \
-    prompt8_kernel<DV, QTV><<<(int)(items * pieces), 256, 0, stream>>>(a, units_z, compute_units(), how);          \
-    if (pieces > 1) prompt8_merge_kernel<DV, QTV><<<dim3((int)items, DV / 32), 256, 0, stream>>>(a, units_z, how); \
+    prompt8_kernel<DV, QTV><<<(int)(items * pieces), 256, 0, stream>>>(a, z, pass, by_pieces, how);                \
+    if (pieces > 1) prompt8_merge_kernel<DV, QTV><<<dim3((int)items, DV / 32), 256, 0, stream>>>(a, z, how);       \
   }
 #define LAUNCH(DV) if (query_tiles == 1) LAUNCH2(DV, 1) else LAUNCH2(DV, 2)
   FOR_WIDTH(LAUNCH)
