@@ -948,23 +948,30 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a
 }
 
 // The partitions of every (token, head): sum acc_p 2^(m_p - m) / sum l_p 2^(m_p - m).  A lane holds a partition's weight and hands it round by lane
-// reads: one round of loads for the weights and one, which waits for no other, for the sums.  A thread has a coordinate (D is whole waves).
+// reads; maxima, sums and the first eight outputs are asked for at once, and nothing waits for another.  A thread has a coordinate (D is whole waves).
 __global__ __launch_bounds__(256) void single8_merge_kernel(Attend a, int D) {
   const int item = blockIdx.x, h = blockIdx.y, t = a.items ? a.items[item] : item, lane = threadIdx.x & (WAVE - 1), d = threadIdx.x;
   const size_t base = ((size_t)item * a.H + h) * a.P;
-  float m = NEG_INF;
-  for (int p = lane; p < a.P; p += WAVE) m = fmaxf(m, a.part_m[base + p]);
-  m = wave_max(m);
   const float* acc = a.part_acc + base * D + d;
+  float v[8];
+  auto ask = [&](int p) {  // eight at a time; those past the end repeat the last with a weight of 0
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = acc[(size_t)min(p + j, a.P - 1) * D];
+  };
+  ask(0);
+  float mp = lane < a.P ? a.part_m[base + lane] : NEG_INF, lp = lane < a.P ? a.part_l[base + lane] : 0.f, m = mp;
+  for (int p = lane + WAVE; p < a.P; p += WAVE) m = fmaxf(m, a.part_m[base + p]);
+  m = wave_max(m);
   float num = 0.f, den = 0.f;
   for (int p0 = 0; p0 < a.P; p0 += WAVE) {
+    if (p0 > 0) {
+      mp = p0 + lane < a.P ? a.part_m[base + p0 + lane] : NEG_INF;
+      lp = p0 + lane < a.P ? a.part_l[base + p0 + lane] : 0.f;
+    }
+    const float weight = mp == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(mp - m), l = weight == 0.f ? 0.f : lp * weight;
     const int here = min(WAVE, a.P - p0);
-    const float mp = lane < here ? a.part_m[base + p0 + lane] : NEG_INF;
-    const float weight = mp == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(mp - m), l = weight == 0.f ? 0.f : a.part_l[base + p0 + lane] * weight;
-    for (int p = 0; p < here; p += 8) {  // eight at a time; those past the end repeat the last with a weight of 0
-      float v[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = acc[(size_t)(p0 + min(p + j, here - 1)) * D];
+    for (int p = 0; p < here; p += 8) {
+      if (p0 + p > 0) ask(p0 + p);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         den += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(l), p + j));
