@@ -66,7 +66,7 @@ __device__ __forceinline__ size_t block_index(const Pages& p, int page, int kvh,
 // block, so that a coordinate's bytes are neighbours in a lane's hands: they cross to the transposed block through LDS.
 //
 // Bound by memory where there is much of it (a prompt of 2,048 tokens, 32 heads of 128 on 8: 11.4 us, 47 MB at 4.2 TB/s; 16-bit pages 12.7) and by a launch
-// and three dependent waits (slots, scale, stores) where there is not: one token 3.0 us, 64 requests' tokens 4.0, 2.6 of it the queries.
+// and three dependent waits (slots, scale, stores) where there is not: one token 3.0 us, 64 requests' tokens 3.8, 2.6 of it the queries.
 template <int D> struct Lanes {
   static constexpr int LPT = D <= 64 ? 8 : D <= 128 ? 16 : 32;  // lanes of a head, D / 8 of them busy
   static constexpr int AT_ONCE = WAVE / LPT, PASSES = BLOCK / AT_ONCE;
@@ -769,11 +769,11 @@ __device__ __forceinline__ void insert(Held<D>& held, const News<D>& news, int n
 // One workgroup per (token, group of query heads, partition of its keys); its four waves take the steps in turn.  W: of FRESH, the gains' type.
 //
 // Bound by the pages' bytes as soon as there are enough of them: 64 contexts of 300 to 8,000 tokens (32 heads of 128 on 8) 80 to 82 us, 6.6 TB/s (a large
-// copy reads and writes 5.1); one of 131,005 (64 heads on 8) 46 us with its merge, 5.9 TB/s.  16-bit pages: 181 and 83.  A step's operands go from memory into
+// copy reads and writes 5.1); one of 131,005 (64 heads on 8) 45 us with its merge, 5.9 TB/s.  16-bit pages: 183 and 84.  A step's operands go from memory into
 // registers in the order in which the matrix instructions take them: LDS would hold the same bytes once more, and nobody shares them, since all heads of a
 // group are columns of one wave.  Two steps in flight a wave (one being taken, one on its way) hide most of the latency: the
 // form that loaded a step when it came to it took 252 us for the 64 contexts.
-// Where there is little to read, latency is the bound: 700 keys of one request 7.0 us (16-bit pages 6.7), of which a launch, the page's entry, the
+// Where there is little to read, latency is the bound: 700 keys of one request 6.4 us (16-bit pages 6.6), of which a launch, the page's entry, the
 // operands and the exchange between waves wait for one another.
 template <int D, bool FRESH, typename W>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a, Fresh fresh) {

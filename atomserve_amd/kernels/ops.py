@@ -929,7 +929,7 @@ def _up64(n: int) -> int:
 # and how many workgroups a compute unit has at once.  A step lasts as long as a workgroup, or as all of them take their places, and no less than memory
 # (7.3 TB/s) needs; the merge is 1.6 us, 0.04 a partition and 2.3 TB/s for what partitions leave.  From one and a half (token, kv head) pairs a compute
 # unit on contexts stay whole, which many requests of unequal length want.  What it picks takes 1.3 per cent more than the best of eight sizes on
-# average and 20 at worst (the rule of 16-bit pages, 4.5 and 54).
+# average and 9 at worst (the rule of 16-bit pages, 4.5 and 54).
 SINGLE8_COSTS = {64: (4.1, 0.0033, 4.4), 128: (4.7, 0.0055, 2.66), 192: (5.2, 0.0084, 1.1), 256: (5.7, 0.0113, 1.1)}
 SINGLE8_PARTITIONS = (128, 256, 512, 1024, 2048, 4096, 8192)
 
@@ -1019,12 +1019,12 @@ def attn_single_query8(q, k_pages, v_pages, k_scales, v_scales, items, positions
 
 def attn_decode_fresh8_supported(dtype, num_heads: int, num_kv_heads: int, head_dim: int, block_size: int, rotary_dim: int) -> bool:
     """Whether `attn_decode_fresh8` takes this case: what `cache8_supported` names, at most 16 query heads to a kv head, heads of up to 192.  us of the one
-    kernel / of the two, heads of 128 (32 on 8), 64 (16 on 4), 192 (24 on 8), by requests x tokens (heads of 256, 8 on 4, whose operands fill the registers:
-    10.6/10.3, 13.2/13.0, 15.6/17.5, 54.8/50.2, 45.5/37.7; not taken):
+    kernel / of the two, heads of 128 (32 on 8), 64 (16 on 4), 192 (24 on 8), by requests x tokens (heads of 256, 8 on 4, whose operands fill the registers,
+    lost a tenth at 64 and more requests; not taken):
         1 x 100       1 x 2,000     8 x 2,048     64 x 2,048    128 x 500
-        8.0/8.7       10.5/11.3     13.2/14.5     45.0/46.5     32.8/31.9
-        6.5/7.7       8.9/10.2      8.7/10.4      16.9/17.6     10.4/11.6
-        9.6/9.8       12.3/12.5     17.8/19.0     69.3/69.2     57.6/52.2"""
+        6.4/8.2       8.8/10.8      11.2/13.1     42.7/45.0     29.8/29.7
+        5.7/7.3       7.7/9.6       7.7/9.4       16.0/17.3     9.6/11.5
+        7.4/9.2       9.9/11.7      15.6/18.2     68.4/67.8     52.0/49.5"""
     return (cache8_supported(dtype, num_heads, num_kv_heads, head_dim, block_size, rotary_dim) and num_heads // num_kv_heads <= 16
             and head_dim <= 192)  # fmt: skip
 
