@@ -1020,7 +1020,7 @@ def attn_single_query8(q, k_pages, v_pages, k_scales, v_scales, items, positions
 def attn_decode_fresh8_supported(dtype, num_heads: int, num_kv_heads: int, head_dim: int, block_size: int, rotary_dim: int) -> bool:
     """Whether `attn_decode_fresh8` takes this case: what `cache8_supported` names, at most 16 query heads to a kv head, heads of up to 192.  us of the one
     kernel / of the two, heads of 128 (32 on 8), 64 (16 on 4), 192 (24 on 8), by requests x tokens (heads of 256, 8 on 4, whose operands fill the registers,
-    lost a tenth at 64 and more requests; not taken):
+    lost a tenth and more at 64 and more requests; not taken):
         1 x 100       1 x 2,000     8 x 2,048     64 x 2,048    128 x 500
         6.4/8.2       8.8/10.8      11.2/13.1     42.7/45.0     29.8/29.7
         5.7/7.3       7.7/9.6       7.7/9.4       16.0/17.3     9.6/11.5

@@ -268,3 +268,44 @@ def test_a_step_whose_queries_see_nothing(ops):
         out.fill_(7.0)
         ops.attn_decode_fresh8(s.next_qkv, *s.gains, s.next_cos_sin, none, 1e-6, True, *s.cache, none, s.tables, out, s.H, 0.1, 0, 0, part_size=part)
         assert not bool(out.any()) and same(s.state()[3:], before)
+
+
+def test_many_tokens(ops):
+    """70,001 single queries, and as many tokens of portions, in one call: the results of calls of a thousand."""
+    H, KV, D, bs, T = 6, 3, 64, 16, 70_001
+    g = torch.Generator(device=DEV).manual_seed(0)
+    cache = plain.empty(30, KV, bs, D, DEV)
+    plain.fill(cache, *(torch.randn(30, KV, bs, D, generator=g, device=DEV) for _ in range(2)))
+    q = torch.randn(T, H, D, generator=g, device=DEV).to(BF16)
+    tables = i32([list(range(r, r + 10)) for r in (0, 10, 20)])
+    positions, rows = torch.randint(-1, 150, (T,), generator=g, device=DEV, dtype=I32), torch.randint(0, 3, (T,), generator=g, device=DEV, dtype=I32)
+    whole, cut = torch.empty_like(q), torch.empty_like(q)
+    ops.attn_single_query8(q, *cache, None, positions, rows, tables, whole, 0.125, 0, 150, part_size=192)
+    for at in range(0, T, 1000):
+        part = slice(at, min(at + 1000, T))
+        ops.attn_single_query8(q[part], *cache, None, positions[part], rows[part], tables, cut[part], 0.125, 0, 150, part_size=192)
+    assert torch.equal(whole, cut)
+    tiles = [(at, min(64, T - at), at % 3, at % 90) for at in range(0, T, 64)]
+    ops.attn_prefill8(q, *cache, i32(tiles), tables, whole, 0.125, 0, 154, query_tiles=1)
+    for at in range(0, len(tiles), 16):
+        ops.attn_prefill8(q, *cache, i32(tiles[at : at + 16]), tables, cut, 0.125, 0, 154, query_tiles=1)
+    assert torch.equal(whole, cut)
+
+
+def test_many_tokens_appended(ops):
+    """70,001 tokens in one call, runs and single tokens and some that are not kept: the bytes of calls of a thousand."""
+    H, KV, D, bs, T = 2, 3, 64, 16, 70_001
+    g = torch.Generator(device=DEV).manual_seed(0)
+    qkv = torch.randn(T, H + 2 * KV, D, generator=g, device=DEV).to(BF16)
+    cos_sin = torch.randn(T, D // 2, 2, generator=g, device=DEV)
+    slots = torch.arange(T, device=DEV, dtype=I32)
+    slots[40_000:] = (40_000 // 16 + torch.arange(T - 40_000, device=DEV, dtype=I32)) * 16 + 7  # from here on single tokens, each in a block of its own
+    slots[torch.randint(0, T // 16, (500,), generator=g, device=DEV) * 16 + 15] = -1
+    one, many = (plain.empty(40_000 // 16 + T - 40_000, KV, bs, D, DEV) for _ in range(2))
+    queries = [torch.empty(T, H, D, dtype=BF16, device=DEV) for _ in range(2)]
+    ops.qk_norm_rope_store8(qkv, None, None, cos_sin, slots, queries[0], *one, H, KV, 0.0)
+    for at in range(0, T, 1008):
+        part = slice(at, min(at + 1008, T))
+        ops.qk_norm_rope_store8(qkv[part], None, None, cos_sin[part], slots[part], queries[1][part], *many, H, KV, 0.0)
+    assert torch.equal(*queries) and all(same([a.view(torch.uint8) if a.element_size() == 1 else a], [b.view(torch.uint8) if b.element_size() == 1 else b])
+                                         for a, b in zip(one, many))  # fmt: skip
