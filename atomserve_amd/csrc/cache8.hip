@@ -421,6 +421,8 @@ template <int D> struct Query {
   float scale;
 };
 
+constexpr unsigned FOUR_NANS = 0x7f7f7f7fu;  // what a query that is not finite is made of: its scores become NaN, and none of its neighbours'
+
 // Four numbers of a query, scaled, as their two parts.
 __device__ __forceinline__ void split4(const float* x, float inv, unsigned& high, unsigned& low) {
   float y[4];
@@ -445,16 +447,16 @@ template <int D> __device__ __forceinline__ void load_query(Query<D>& q, const b
   const float amax = quad_rows_max(__uint_as_float(min(most, 0x7f800000u)));
   q.scale = block_scale(amax);
   const float inv = inverse_of(q.scale);
+  const bool finite = amax < __builtin_inff();
 #pragma unroll
   for (int c = 0; c < D / 64; ++c)
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       unsigned high, low;
       split4(x[c] + 4 * w, inv, high, low);
-      q.high[c][w] = high;
+      q.high[c][w] = finite ? high : FOUR_NANS;
       q.low[c][w] = low;
     }
-  if (amax == __builtin_inff()) q.scale = __builtin_nanf("");  // no e4m3 number stands for it: what it sees becomes NaN, and none of its neighbours
 }
 
 __device__ __forceinline__ i32x8_t both(u32x4_t a, u32x4_t b) {
@@ -562,7 +564,12 @@ __device__ __forceinline__ float max_of_16(const f32x4_t (&s)[4]) {
   return max3(max3(m0, m1, m2), max3(m3, m4, s[3][3]), NEG_INF);
 }
 
-// A step's products and softmax for queries of one token (pos, lo uniform).  factor: from a score of e4m3 numbers to one in base 2 (natural units where
+// What a score of e4m3 numbers is multiplied by: the query's factor times the block's scale, 0 of a block that was never written.  Kept a normal number:
+// either is as small as 2^-100 where all is zero, and a scale can be that of keys that are hidden, but a hidden score's -inf times 0, or a score of 0 times
+// infinity, would be NaN.
+__device__ __forceinline__ float score_unit(float factor, float scale) { return __builtin_amdgcn_fmed3f(factor * scale, 0x1p-126f, 0x1.fffffep127f); }
+
+// A step's products and softmax for queries of one token (pos, lo uniform).  factor: from a score of e4m3 numbers to one in base 2 (to one in caps where
 // scores are capped), without the block's scale.
 template <int D>
 __device__ __forceinline__ void take_step(const Held<D>& held, int kb, const Query<D>& q, float factor, float cap, int pos, int lo, int keep,
@@ -571,9 +578,8 @@ __device__ __forceinline__ void take_step(const Held<D>& held, int kb, const Que
   f32x4_t s[4];
 #pragma unroll
   for (int tt = 0; tt < 4; ++tt) s[tt] = score_tile<D>(held.k[tt], q);
-  float by = factor * fmaxf(held.ks, 0x1p-100f);  // a block that was never written has none; -inf times it stays -inf
+  float by = score_unit(factor, held.ks);
   if (cap > 0.f) {  // uniform
-    by *= __builtin_amdgcn_rcpf(cap);
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
@@ -665,7 +671,7 @@ struct Attend {
   Divide kv, group;  // by KV and H / KV
 };
 
-__device__ __forceinline__ float score_factor(const Attend& a) { return a.sight.cap > 0.f ? a.scale : a.scale * LOG2E; }
+__device__ __forceinline__ float score_factor(const Attend& a) { return a.scale * (a.sight.cap > 0.f ? __builtin_amdgcn_rcpf(a.sight.cap) : LOG2E); }
 
 // The weighted sum over its denominator; nothing seen: 0.  m in base 2.
 __device__ __forceinline__ float share_of(const Sight& sight, int head, float m, float l) {
@@ -862,9 +868,15 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a
         const float amax = lanes_max<LPT>(busy ? __uint_as_float(min(most, 0x7f800000u)) : 0.f), scale = block_scale(amax), inv = inverse_of(scale);
         if (!busy) continue;
         Split<D>& to8 = queries[job];
-        split4(x, inv, to8.high[at8.a / 4], to8.low[at8.a / 4]);
-        split4(x + 4, inv, to8.high[at8.b / 4], to8.low[at8.b / 4]);
-        if (j == 0) to8.scale = amax == __builtin_inff() ? __builtin_nanf("") : scale;
+        unsigned high[2], low[2];
+        split4(x, inv, high[0], low[0]);
+        split4(x + 4, inv, high[1], low[1]);
+        const bool finite = amax < __builtin_inff();
+        to8.high[at8.a / 4] = finite ? high[0] : FOUR_NANS;
+        to8.high[at8.b / 4] = finite ? high[1] : FOUR_NANS;
+        to8.low[at8.a / 4] = low[0];
+        to8.low[at8.b / 4] = low[1];
+        if (j == 0) to8.scale = scale;
       } else {
         float amax = 0.f;
 #pragma unroll
@@ -1208,9 +1220,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt8_kernel(Attend a
       bool grows = false;
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
-        by[qt] = factor[qt] * fmaxf(ks, 0x1p-100f);
+        by[qt] = score_unit(factor[qt], ks);
         if (a.sight.cap > 0.f) {
-          by[qt] *= __builtin_amdgcn_rcpf(a.sight.cap);
 #pragma unroll
           for (int tt = 0; tt < 4; ++tt)
 #pragma unroll

@@ -1,0 +1,152 @@
+"""The kernels of the cache in 8 bits where numbers are zero, far apart or at a scale's border, against plain 64-bit forms (tests/plain_cache8.py)."""
+
+import pytest
+import torch
+
+from tests import plain_cache8 as plain
+
+pytestmark = pytest.mark.gpu
+F32, F64, BF16, I32, DEV = torch.float32, torch.float64, torch.bfloat16, torch.int32, "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from atomserve_amd.kernels import ops as module
+
+    return module
+
+
+def i32(values):
+    return torch.tensor(values, dtype=I32, device=DEV)
+
+
+# ---- scores' factors that 32 bits do not hold ---------------------------------------------------------
+
+
+def one_request(L, H, KV, D, bs, keys, filler=3):
+    """A cache whose pages, in order, are one request of L tokens and `filler` pages that were never written, its table [1, W] with entries that name
+    those behind the request's, and keys [L, KV, D] as given beside values of a few units."""
+    need = -(-L // bs)
+    cache = plain.empty(need + filler, KV, bs, D, DEV)
+    g = torch.Generator(device=DEV).manual_seed(L * 1000 + D)
+    k, v = (torch.zeros(need * bs, KV, D, device=DEV) for _ in range(2))
+    k[:L] = keys
+    v[:L] = torch.randn(L, KV, D, generator=g, device=DEV) + 2.0
+    used = tuple(x[:need] for x in cache)
+    plain.fill(used, *(x.view(need, bs, KV, D).transpose(1, 2).contiguous() for x in (k, v)))
+    for scales in used[2:]:  # blocks behind the last token were never written either
+        scales.view(need, KV, -1)[-1, :, ((L - 1) % bs) // 16 + 1 :] = 0.0
+    return cache, [*range(need), *range(need, need + filler)]
+
+
+def check_all(ops, monkeypatch, q, cache, table, visible=None, **kw):
+    """Queries q [L, H, D] of one request, each at its own position: as single queries, whole and in partitions, and as portions, whole and cut."""
+    L, H, D = q.shape
+    scale, tables, positions = plain.default_scale(D), i32([table]), i32(range(L))
+    k, v = plain.gathered(cache, table, L)
+    sink = kw.get("sink", False)
+    sink = sink if isinstance(sink, torch.Tensor) else torch.zeros(H, device=DEV) if sink else None
+    rows = range(L) if visible is None else range(visible)
+    want, bound = zip(*[plain.attend(q[p], k[:, : p + 1], v[:, : p + 1], p, scale, cap=kw.get("softcap", 0.0), sink=sink) for p in rows])
+    want, bound = torch.stack(want), torch.stack(bound)
+
+    def check(out, name):
+        off = (out[: len(rows)].double() - want).abs()
+        assert bool((off <= bound).all()), (name, float((off - bound).nan_to_num(nan=float("inf")).max()))
+
+    for part in (64, 4096):
+        out = torch.full_like(q, 7.0)
+        ops.attn_single_query8(q, *cache, None, positions, torch.zeros(L, dtype=I32, device=DEV), tables, out, scale, 0, L, part_size=part, **kw)
+        check(out, f"partitions of {part}")
+    tiles = i32([(at, min(64, L - at), 0, at) for at in range(0, L, 64)])
+    for query_tiles in (1, 2):
+        for pieces in (1, 2):
+            monkeypatch.setattr(ops, "PREFILL_PIECES", pieces)
+            out = torch.full_like(q, 7.0)
+            ops.attn_prefill8(q, *cache, tiles, tables, out, scale, 0, L, query_tiles=query_tiles, **kw)
+            check(out, f"{query_tiles} tiles a wave, {pieces} pieces")
+
+
+SEES = [{}, {"softcap": 8.0}, {"softcap": 0.25}, {"sink": True}]
+
+
+@pytest.mark.parametrize("kw", SEES, ids=str)
+@pytest.mark.parametrize("D,bs", [(64, 16), (128, 64), (192, 16), (256, 32)])
+@pytest.mark.parametrize("L", [1, 5, 17, 63, 130])
+@pytest.mark.parametrize("keys", ["zero", "small", "units"])
+def test_queries_of_zeros_see_the_mean_of_the_values(ops, monkeypatch, D, bs, L, keys, kw):
+    """Beside keys that are zeros (a padding token's), so small that they are stored as zeros, and ordinary ones, with blocks behind the last token that were
+    never written: every visible key weighs the same."""
+    H, KV = 4, 2
+    size = {"zero": 0.0, "small": 1e-37, "units": 1.0}[keys]
+    cache, table = one_request(L, H, KV, D, bs, torch.randn(L, KV, D, device=DEV) * size)
+    check_all(ops, monkeypatch, torch.zeros(L, H, D, dtype=BF16, device=DEV), cache, table, **kw)
+    mixed = torch.randn(L, H, D, device=DEV).to(BF16)  # a head of zeros beside others, and tokens of zeros among others
+    mixed[:, 1] = 0
+    mixed[::3] = 0
+    check_all(ops, monkeypatch, mixed, cache, table, **kw)
+
+
+@pytest.mark.parametrize("kw", SEES, ids=str)
+@pytest.mark.parametrize("D", [64, 128, 192])
+def test_a_key_that_is_not_seen_yet_is_far_larger_than_all_that_is(ops, monkeypatch, D, kw):
+    """Its block's scale times a large query's is beyond 32 bits, and the keys that are seen are zeros."""
+    L, H, KV = 12, 4, 2
+    keys = torch.zeros(L, KV, D, device=DEV)
+    keys[8:] = 2.0**120
+    cache, table = one_request(L, H, KV, D, 16, keys)
+    check_all(ops, monkeypatch, torch.full((L, H, D), 2.0**40, device=DEV).to(BF16), cache, table, visible=8, **kw)
+
+
+@pytest.mark.parametrize("D", [64, 128, 192])
+@pytest.mark.parametrize("context", [1, 2, 16, 17, 64, 70])
+def test_a_decode_step_of_zeros(ops, D, context):
+    """Queries and the new key are zeros, from the projection on: the mean of the values, the new one among them."""
+    H, KV, bs = 4, 2, 16
+    cache, table = one_request(context, H, KV, D, bs, torch.zeros(context, KV, D, device=DEV))
+    p = context - 1
+    qkv = torch.zeros(1, H + 2 * KV, D, dtype=BF16, device=DEV)
+    qkv[:, H + KV :] = 3.0
+    cos_sin, slot, scale = plain.positions_angles([p], D).to(DEV), i32([table[p // bs] * bs + p % bs]), plain.default_scale(D)
+    for gains in ([None, None], [torch.ones(D, device=DEV)] * 2):
+        for part in (None, 64):
+            out = torch.full((1, H, D), 7.0, dtype=BF16, device=DEV)
+            ops.attn_decode_fresh8(qkv, *gains, cos_sin, slot, 1e-6, True, *cache, i32([p]), i32([table]), out, H, scale, 0, context, part_size=part)
+            k, v = plain.gathered(cache, table, context)
+            want, bound = plain.attend(torch.zeros(H, D, device=DEV), k, v, p, scale)
+            assert bool(((out[0].double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("keys", ["zero", "units"])
+@pytest.mark.parametrize("kw", [{}, {"softcap": 8.0}, {"sink": True}], ids=str)
+@pytest.mark.parametrize("D", [64, 128, 192, 256])
+def test_queries_that_are_not_finite_are_nan_and_their_neighbours_are_not(ops, monkeypatch, D, kw, keys):
+    """Of every width, at any coordinate, beside keys of zeros too; decode steps from the projection as well."""
+    L, H, KV, bs = 70, 4, 2, 16
+    cache, table = one_request(L, H, KV, D, bs, torch.randn(L, KV, D, device=DEV) * (keys == "units"))
+    q = torch.randn(L, H, D, device=DEV).to(BF16)
+    bad, hit = q.clone(), torch.zeros(L, H, dtype=torch.bool, device=DEV)
+    for i, (t, h, d) in enumerate([(0, 0, 0), (5, 1, D // 2), (16, 2, D - 1), (63, 3, 17), (69, 0, D - 40)]):
+        bad[t, h, d] = (float("nan"), float("inf"), -float("inf"))[i % 3]
+        hit[t, h] = True
+    tables, scale = i32([table]), plain.default_scale(D)
+    tiles = i32([(0, 64, 0, 0), (64, 6, 0, 64)])
+
+    def check(call, x, y, hit):
+        clean, got = (torch.full(q.shape[:1] + (H, D), 7.0, dtype=BF16, device=DEV) for _ in range(2))
+        call(x, clean)
+        call(y, got)
+        assert bool(got[hit].isnan().all()) and bool(clean.isfinite().all()) and torch.equal(got[~hit], clean[~hit])
+
+    for part in (64, 4096):
+        check(lambda x, out: ops.attn_single_query8(x, *cache, None, i32(range(L)), torch.zeros(L, dtype=I32, device=DEV), tables, out, scale, 0, L,
+                                                    part_size=part, **kw), q, bad, hit)  # fmt: skip
+    for query_tiles, pieces in ((1, 1), (2, 2)):
+        monkeypatch.setattr(ops, "PREFILL_PIECES", pieces)
+        check(lambda x, out: ops.attn_prefill8(x, *cache, tiles, tables, out, scale, 0, L, query_tiles=query_tiles, **kw), q, bad, hit)
+    if D <= 192 and not kw:
+        own = lambda x: torch.cat([x, torch.zeros(L, 2 * KV, D, dtype=BF16, device=DEV)], 1)  # noqa: E731
+        nowhere = torch.full((L,), -1, dtype=I32, device=DEV)
+        for part in (64, 4096):
+            check(lambda x, out: ops.attn_decode_fresh8(own(x), None, None, None, nowhere, 0.0, True, *cache, i32(range(L)), tables.expand(L, -1).contiguous(),
+                                                        out, H, scale, 0, L, part_size=part), q, bad, hit)  # fmt: skip
