@@ -124,10 +124,12 @@ struct Places {
   }
 };
 
-// Norm (gains g, or none) and rotation of a head's eight coordinates in this lane by the angles of token t.  busy: the lane has coordinates of its own.
+// Norm (gains g, or none) and rotation of a head's eight coordinates in this lane by the angles of token t.  busy: the lane has coordinates of its own;
+// one that has none holds lane 0's, which are turned as there: largest magnitudes are taken over all lanes.
 template <int D>
 __device__ __forceinline__ void norm_turn(float (&x)[8], bool norm, const float (&g)[8], const float2* cs, float eps, int R, int t, int j, bool busy) {
-  const bool turns = busy && 8 * j < R;
+  if (!busy) j = 0;
+  const bool turns = 8 * j < R;
   float4 a, b;
   if (turns) {
     const float4* angles = reinterpret_cast<const float4*>(cs + (size_t)t * (R / 2) + 4 * j);

@@ -150,3 +150,76 @@ def test_queries_that_are_not_finite_are_nan_and_their_neighbours_are_not(ops, m
         for part in (64, 4096):
             check(lambda x, out: ops.attn_decode_fresh8(own(x), None, None, None, nowhere, 0.0, True, *cache, i32(range(L)), tables.expand(L, -1).contiguous(),
                                                         out, H, scale, 0, L, part_size=part), q, bad, hit)  # fmt: skip
+
+
+# ---- heads whose lanes are not all at work --------------------------------------------------------------
+
+
+def lone_scales(ops, H, KV, D, R, x, gains, tokens):
+    """Scales of the keys and values of one block, filled from its first place on in the three ways there are: [run, single tokens, decode steps]."""
+    bs, c = 16, 0.5**0.5
+    cos_sin = torch.full((tokens, R // 2, 2), c, device=DEV) if R else None
+    qkv = x.to(BF16).expand(tokens, H + 2 * KV, D).contiguous()
+    q = torch.empty(tokens, H, D, dtype=BF16, device=DEV)
+    found = []
+    for how in ("run", "singles", "steps"):
+        cache = plain.empty(2, KV, bs, D, DEV)
+        if how == "run":
+            ops.qk_norm_rope_store8(qkv, *gains, cos_sin, i32(range(tokens)), q, *cache, H, KV, 1e-6)
+        for t in range(tokens):
+            one = slice(t, t + 1)
+            angles = None if cos_sin is None else cos_sin[one]
+            if how == "singles":
+                ops.qk_norm_rope_store8(qkv[one], *gains, angles, i32([t]), q[one], *cache, H, KV, 1e-6)
+            elif how == "steps":
+                ops.attn_decode_fresh8(qkv[one], *gains, angles, i32([t]), 1e-6, True, *cache, i32([t]), i32([[0, 1]]), q[one], H, 0.1, 0, 16)
+        found.append(cache)
+    return found
+
+
+@pytest.mark.parametrize("D,R", [(64, 64), (128, 128), (128, 64), (192, 192), (192, 96), (192, 8), (192, 0)])
+@pytest.mark.parametrize("tokens", [1, 5, 16])
+def test_scales_are_those_of_the_turned_keys(ops, D, R, tokens):
+    """A pair (500, 0) turned by an eighth of a circle is (354, 354), which scale 1 holds; 500 itself would need 2, and so does a value of 500.  With a norm,
+    and with the pair in the last turned place, the same."""
+    H, KV = 4, 2
+    for at in sorted({0, 3, max(R // 2 - 1, 0)}):
+        x = torch.full((D,), 0.25, device=DEV)
+        x[at] = 500.0
+        if R:
+            x[at + R // 2] = 0.0
+        gains = torch.full((D,), 500.0 / D**0.5, device=DEV)
+        rms = (x.to(BF16).double().square().mean() + 1e-6).sqrt()
+        for norm in ([None, None], [gains, gains]):
+            turned = x.to(BF16).double() if norm[0] is None else x.to(BF16).double() / rms * gains.double()
+            if R:
+                a, b = turned[: R // 2].clone(), turned[R // 2 : R].clone()
+                turned[: R // 2], turned[R // 2 : R] = (a - b) * 0.5**0.5, (b + a) * 0.5**0.5
+            want = plain.scale_of(float(turned.abs().amax()))
+            for cache in lone_scales(ops, H, KV, D, R, x, norm, tokens):
+                assert cache[2][0].flatten().tolist() == [want] * KV and cache[3][0].flatten().tolist() == [2.0] * KV
+                held = plain.keys_of(cache[0], cache[2])[0, :, :tokens]
+                step = torch.maximum(turned.abs() * plain.HALF_STEP, torch.tensor(plain.SMALLEST_HALF_STEP * want, dtype=F64, device=DEV))
+                assert bool(((held - turned).abs() <= step + 2.0**-18 * turned.abs().amax()).all())
+
+
+@pytest.mark.parametrize("R", [192, 96])
+def test_scales_of_many_turned_heads_of_192(ops, R):
+    """4,096 blocks of one token, without norms: the scale of the largest turned coordinate.  In 32 bits a c - b s is off by at most 2^-24 (|a c| + |b s|) for
+    each of two roundings and the table's own, and |a c| + |b s| is at most twice the larger of the pair's turned coordinates: by less than 2^-20 of the largest
+    in all, within which of a border either scale is right."""
+    H, KV, D, T = 1, 2, 192, 4096
+    g = torch.Generator(device=DEV).manual_seed(1)
+    qkv = torch.randn(T, H + 2 * KV, D, generator=g, device=DEV).to(BF16)
+    angles = torch.rand(T, R // 2, generator=g, device=DEV) * 6.28
+    cos_sin = torch.stack([angles.cos(), angles.sin()], -1)
+    cache = plain.empty(T, KV, 16, D, DEV)
+    q = torch.empty(T, H, D, dtype=BF16, device=DEV)
+    ops.qk_norm_rope_store8(qkv, None, None, cos_sin, torch.arange(T, dtype=I32, device=DEV) * 16, q, *cache, H, KV, 0.0)
+    k = qkv[:, H : H + KV].double()
+    c, s = (cos_sin[..., i].double()[:, None] for i in range(2))
+    a, b = k[..., : R // 2], k[..., R // 2 : R]
+    amax = torch.cat([a * c - b * s, b * c + a * s, k[..., R:]], -1).abs().amax(-1).cpu()
+    low, high = ([[plain.scale_of(float(x)) for x in row] for row in amax * f] for f in (1 - 2.0**-20, 1 + 2.0**-20))
+    got = cache[2][..., 0].cpu()
+    assert bool(((got == torch.tensor(low)) | (got == torch.tensor(high))).all())
