@@ -679,6 +679,7 @@ __device__ __forceinline__ float score_factor(const Attend& a) { return a.scale 
 __device__ __forceinline__ float share_of(const Sight& sight, int head, float m, float l) {
   if (sight.sink) {
     const float sk = sink_score(1, sight.sinks, head) * LOG2E, top = fmaxf(m, sk), e = __builtin_amdgcn_exp2f(m - top);
+    if (top == NEG_INF) return 0.f;  // a sink of no weight, beside nothing
     return e / (l * e + __builtin_amdgcn_exp2f(sk - top));
   }
   return l > 0.f ? 1.0f / l : 0.f;

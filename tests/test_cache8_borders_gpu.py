@@ -223,3 +223,24 @@ def test_scales_of_many_turned_heads_of_192(ops, R):
     low, high = ([[plain.scale_of(float(x)) for x in row] for row in amax * f] for f in (1 - 2.0**-20, 1 + 2.0**-20))
     got = cache[2][..., 0].cpu()
     assert bool(((got == torch.tensor(low)) | (got == torch.tensor(high))).all())
+
+
+# ---- a sink of no weight -----------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("lowest", [-float("inf"), torch.finfo(F32).min])
+@pytest.mark.parametrize("part", [64, 512])
+def test_a_query_that_sees_nothing_beside_a_sink_of_no_weight_is_zero(ops, lowest, part):
+    """Heads whose sink is -inf, or the lowest number, have none: a query that sees keys is attention without it, one that sees nothing zeros."""
+    H, KV, D, bs, L = 4, 2, 64, 16, 200
+    cache, table = one_request(L, H, KV, D, bs, torch.randn(L, KV, D, device=DEV))
+    q = torch.randn(3, H, D, device=DEV).to(BF16)
+    sink = torch.tensor([lowest, 0.5, lowest, -3.0], device=DEV)
+    out, scale = torch.full_like(q, 7.0), plain.default_scale(D)
+    positions = [-1, 199, 20]
+    ops.attn_single_query8(q, *cache, None, i32(positions), i32([0, 0, 0]), i32([table]), out, scale, 0, L, part_size=part, sink=sink)
+    assert not bool(out[0].any())
+    k, v = plain.gathered(cache, table, L)
+    for t in (1, 2):
+        want, bound = plain.attend(q[t], k[:, : positions[t] + 1], v[:, : positions[t] + 1], positions[t], scale, sink=sink)
+        assert bool(((out[t].double() - want).abs() <= bound).all())
