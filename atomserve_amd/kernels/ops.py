@@ -1018,15 +1018,29 @@ def attn_single_query8(q, k_pages, v_pages, k_scales, v_scales, items, positions
 
 
 def attn_decode_fresh8_supported(dtype, num_heads: int, num_kv_heads: int, head_dim: int, block_size: int, rotary_dim: int) -> bool:
-    """Whether `attn_decode_fresh8` takes this case: what `cache8_supported` names, at most 16 query heads to a kv head, heads of up to 192.  us of the one
-    kernel / of the two, heads of 128 (32 on 8), 64 (16 on 4), 192 (24 on 8), by requests x tokens (heads of 256, 8 on 4, whose operands fill the registers,
-    lost a tenth and more at 64 and more requests; not taken):
-        1 x 100       1 x 2,000     8 x 2,048     64 x 2,048    128 x 500
-        6.4/8.2       8.8/10.8      11.2/13.1     42.7/45.0     29.8/29.7
-        5.7/7.3       7.7/9.6       7.7/9.4       16.0/17.3     9.6/11.5
-        7.4/9.2       9.9/11.7      15.6/18.2     68.4/67.8     52.0/49.5"""
+    """Whether `attn_decode_fresh8` takes this case: what `cache8_supported` names, at most 16 query heads to a kv head, heads of up to 192 (heads of 256, 8
+    on 4, whose operands fill the registers, lost a tenth and more at 64 and more requests)."""
     return (cache8_supported(dtype, num_heads, num_kv_heads, head_dim, block_size, rotary_dim) and num_heads // num_kv_heads <= 16
             and head_dim <= 192)  # fmt: skip
+
+
+def decode_fresh8_faster(tokens: int, num_kv_heads: int, head_dim: int, max_context: int) -> bool:
+    """Whether a decode step of so many tokens and contexts of up to max_context is faster through `attn_decode_fresh8` than through append and attention,
+    whose numbers are the same.  The one kernel saves a launch and the queries' way through memory, some 2 to 3 us, but needs more registers, and each of its
+    workgroups, one a (token, kv head) pair and partition, norms and turns its queries before it has keys to wait for: that adds up where
+    workgroups take many turns and, for heads of 192, which have a compute unit to themselves, where keys are many too.  us of the one / of the two:
+
+        requests x tokens             8 x 500    32 x 500   64 x 100   64 x 2,048  128 x 500  256 x 300  512 x 300
+        32 heads of 128 on 8          9.1/11.1   9.8/12.4   8.1/10.9   43.4/45.8   30.3/30.4  44.5/41.4  82.3/70.7
+        16 of 64 on 4                 7.3/8.7    7.6/9.2    6.7/8.4    16.6/17.8   9.8/11.8   16.4/16.4  28.7/25.8
+        24 of 192 on 8                11.1/13.9  14.6/17.5  15.1/17.8  68.9/68.6   53.0/50.7  87.3/80.6  171/155
+
+    Over 318 steps like these (8 to 512 requests, 100 to 16,000 tokens, 1 to 16 kv heads) what this picks takes 0.2 per cent more than the faster one on average
+    and 9 at worst; the one kernel everywhere, 2.7 and 24."""
+    pairs = tokens * num_kv_heads
+    if head_dim <= 128:
+        return pairs < 2048
+    return pairs < 192 or pairs * (max_context + 200) < 600_000
 
 
 def attn_decode_fresh8(qkv, q_weight, k_weight, cos_sin, slots, eps, store_kv, k_pages, v_pages, k_scales, v_scales, positions, block_tables, out,

@@ -115,7 +115,9 @@ class Attention(Mixer):
         eight = getattr(cache, "k_scales", None) is not None
         fresh = None  # a decode step: norm, rotation, the cache store and attention in one kernel
         if eight:
-            if step.decode_only and ops.attn_decode_fresh8_supported(env.dtype, H, KV, D, cache.block_size, rotary):
+            seen = min(step.max_context, s.window) if s.window else step.max_context
+            if (step.decode_only and ops.attn_decode_fresh8_supported(env.dtype, H, KV, D, cache.block_size, rotary)
+                    and ops.decode_fresh8_faster(T, KV, D, seen)):  # fmt: skip
                 fresh = ops.attn_decode_fresh8
         elif step.decode_only and ops.attn_decode_fresh_supported(*case):
             fresh = ops.attn_decode_fresh
