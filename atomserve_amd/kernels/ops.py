@@ -1149,8 +1149,12 @@ def attn_prefill8(q, k_pages, v_pages, k_scales, v_scales, tiles, block_tables, 
         raise KernelError("attention over 8 bits: scores have a positive scale")
     if max_context > table_width * bs:
         raise KernelError("attention: block tables are shorter than the longest context")
-    query_tiles, pieces, piece_rounds = _prefill8_plan(num_tiles, H, KV, D, max_context, window or chunk, query_tiles or PREFILL_QUERY_TILES,
-                                                       tile_keys, PREFILL_PIECES, compute_units(), sight[1])  # fmt: skip
+    if query_tiles is None:
+        query_tiles = PREFILL_QUERY_TILES
+    if query_tiles not in (None, 1, 2):
+        raise KernelError(f"prefill attention over 8 bits: a wave owns 1 or 2 query tiles, not {query_tiles}")
+    query_tiles, pieces, piece_rounds = _prefill8_plan(num_tiles, H, KV, D, max_context, window or chunk, query_tiles, tile_keys, PREFILL_PIECES,
+                                                       compute_units(), sight[1])  # fmt: skip
     parts = None  # outputs, maxima and sums of the pieces, and how many pieces each item has
     if pieces > 1:
         parts = torch.empty(T * H * pieces * (D + 2) + num_tiles * KV * _prefill_units(query_tiles, H // KV), dtype=F32, device=q.device)

@@ -1,0 +1,18 @@
+"""Arguments of the calls over a cache in 8 bits that name no kernel are refused as such, on the host."""
+
+import pytest
+
+from atomserve_amd.kernels import ops
+from tests.test_cache8 import nothing_is_launched, prompt  # noqa: F401 (a fixture that every test here uses)
+
+
+@pytest.mark.parametrize("query_tiles", [0, 3, 4, -1])
+def test_other_numbers_of_query_tiles_are_refused(query_tiles):
+    with pytest.raises(ops.KernelError, match="query tiles"):
+        prompt(query_tiles=query_tiles)
+
+
+@pytest.mark.parametrize("query_tiles", [None, 1, 2])
+def test_one_two_or_a_choice_go_to_the_kernel(query_tiles):
+    with pytest.raises(AssertionError, match="would have been launched"):
+        prompt(query_tiles=query_tiles)
