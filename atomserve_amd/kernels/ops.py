@@ -835,7 +835,7 @@ def _stream8(here: int) -> int:
 
 def _sight8(window, keep_first, chunk, softcap, sink, q, out, here: int) -> tuple:
     """`_sight`, with results and sinks on the current device."""
-    if window == keep_first == chunk == softcap == 0 and sink is False and out.dtype is BF16:  # most calls
+    if window == keep_first == chunk == softcap == 0 and sink is False and getattr(out, "dtype", None) is BF16:  # most calls
         _check8(out, "out", BF16, q.shape, here)
         return 0, 0, 0, 0.0, 0, 0, 0
     sight = _sight(window, keep_first, chunk, softcap, sink, q, out)

@@ -3,7 +3,7 @@
 import pytest
 
 from atomserve_amd.kernels import ops
-from tests.test_cache8 import nothing_is_launched, prompt  # noqa: F401 (a fixture that every test here uses)
+from tests.test_cache8 import nothing_is_launched, prompt, single  # noqa: F401 (a fixture that every test here uses)
 
 
 @pytest.mark.parametrize("query_tiles", [0, 3, 4, -1])
@@ -16,3 +16,10 @@ def test_other_numbers_of_query_tiles_are_refused(query_tiles):
 def test_one_two_or_a_choice_go_to_the_kernel(query_tiles):
     with pytest.raises(AssertionError, match="would have been launched"):
         prompt(query_tiles=query_tiles)
+
+
+@pytest.mark.parametrize("call", [single, prompt])
+@pytest.mark.parametrize("out", [None, 3])
+def test_results_that_are_no_tensor_are_refused(call, out):
+    with pytest.raises(ops.KernelError):
+        call(out=out)
