@@ -1003,7 +1003,7 @@ def attn_single_query8(q, k_pages, v_pages, k_scales, v_scales, items, positions
         raise KernelError(f"attention: {T} tokens that are their own rows need as many block tables")
     if N == 0:
         return
-    if H % KV or width != D:
+    if H == 0 or H % KV or width != D:
         raise KernelError(f"attention over 8 bits: heads {H}/{KV} of {D} do not fit pages of heads of {width}")
     if not scale > 0:
         raise KernelError("attention over 8 bits: scores have a positive scale")

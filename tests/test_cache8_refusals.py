@@ -23,3 +23,8 @@ def test_one_two_or_a_choice_go_to_the_kernel(query_tiles):
 def test_results_that_are_no_tensor_are_refused(call, out):
     with pytest.raises(ops.KernelError):
         call(out=out)
+
+
+def test_single_queries_without_heads_are_refused():
+    with pytest.raises(ops.KernelError, match="heads 0/2"):
+        single(H=0)
