@@ -9,8 +9,10 @@
 // A token at position p of a request lives in page table[p / bs] at offset p % bs, so that a block of either kind is 16 D bytes in one piece, at
 // the same place in both.  A block's scale is the power of two 2^e with the smallest e in -100 .. 119 for which its largest magnitude is at
 // most 448 * 2^e (448 is the largest e4m3 number).  A block is filled token by token while its scale grows, and what it holds is then
-// rewritten: times a power of two an e4m3 number stays the same number unless it falls under the smallest normal one (2^-15 of the
-// largest), so a block holds what a single rounding gives, however its tokens came.  Integers, or any scale, would be rounded anew each time.
+// rewritten: times a power of two an e4m3 number stays the same number unless it falls under the smallest normal one, 2^-6 of the scale (2^-14.8 to
+// 2^-13.8 of the largest).  So a number above that is what a single rounding gives, off by at most 2^-4 of itself, however its tokens came; one below is
+// rounded again at every growth, by half a smallest step of scales that double at least: by at most 2^-9 of the last scale in all.  Integers, or any
+// scale, would be rounded anew each time throughout.
 #include "attn_parts.h"
 #include "wide_tile.h"
 
@@ -66,7 +68,7 @@ __device__ __forceinline__ size_t block_index(const Pages& p, int page, int kvh,
 // block, so that a coordinate's bytes are neighbours in a lane's hands: they cross to the transposed block through LDS.
 //
 // Bound by memory where there is much of it (a prompt of 2,048 tokens, 32 heads of 128 on 8: 11.4 us, 47 MB at 4.2 TB/s; 16-bit pages 12.7) and by a launch
-// and three dependent waits (slots, scale, stores) where there is not: one token 3.0 us, 64 requests' tokens 3.8, 2.6 of it the queries.
+// and three dependent waits (slots, scale, stores) where there is not: one token 3.0 us, 64 requests' tokens 3.8 to 4.0, 2.6 of it the queries.
 template <int D> struct Lanes {
   static constexpr int LPT = D <= 64 ? 8 : D <= 128 ? 16 : 32;  // lanes of a head, D / 8 of them busy
   static constexpr int AT_ONCE = WAVE / LPT, PASSES = BLOCK / AT_ONCE;
@@ -410,9 +412,13 @@ template <int D, typename W> __global__ __launch_bounds__(256) void append8_kern
 //
 //   S^T[key][column] = K Q^T     the e4m3 keys as they are (16x16x128, 8-bit operands).  A query is scaled by a power of two as a block is and
 //                                split in two e4m3 parts, the number rounded and what is left of it: 4 + 4 bits hold a bf16 number's eight
-//                                exactly, down to 2^-10 of the query's largest coordinate, and what is smaller is off by 2^-19 of it at most.
+//                                exactly, down to 2^-9.8 of the query's largest coordinate, and what is smaller is off by 2^-17.8 of it at most
+//                                (half a smallest step, 2^-10, where the largest is 224 or more).
 //   softmax                      fp32, base 2, maxima and sums kept per column
-//   O^T[d][column] += V^T P^T    values as bf16 (exact, the scale included), weights rounded to bf16
+//   O^T[d][column] += V^T P^T    values as bf16 (exact, the scale included), weights rounded to bf16: the matrix cores' operands, a part of 2^-8 at most
+//
+// The denominator is the 32-bit sum of the weights: as they are for single queries, rounded for portions, where the matrix cores add them up.  Either way a
+// result is off by that part of the weighted magnitudes, as over 16-bit pages.
 //
 // Row r of score tile tt (0 .. 3) stands for key 16 (r / 4) + 4 tt + r % 4 of a step, so that the 16 keys whose weights a lane holds after the score
 // product are one block: one scale, and in the transposed values 16 bytes a coordinate.
@@ -782,7 +788,7 @@ __device__ __forceinline__ void insert(Held<D>& held, const News<D>& news, int n
 // registers in the order in which the matrix instructions take them: LDS would hold the same bytes once more, and nobody shares them, since all heads of a
 // group are columns of one wave.  Two steps in flight a wave (one being taken, one on its way) hide most of the latency: the
 // form that loaded a step when it came to it took 252 us for the 64 contexts.
-// Where there is little to read, latency is the bound: 700 keys of one request 6.4 us (16-bit pages 6.6), of which a launch, the page's entry, the
+// Where there is little to read, latency is the bound: 700 keys of one request 6.5 us (16-bit pages 6.6), of which a launch, the page's entry, the
 // operands and the exchange between waves wait for one another.
 template <int D, bool FRESH, typename W>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a, Fresh fresh) {
@@ -1012,7 +1018,7 @@ __global__ __launch_bounds__(256) void single8_merge_kernel(Attend a, int D) {
 //
 // Bound by the matrix cores' products and the softmax between them, at the clock that is left: with QT 2 and heads of 128 a wave's round is 52 products (1,090
 // cycles); matrix cores are busy 57 per cent of the time and the vector unit 49.  Sums of weights are products with ones, which the vector unit would take 128
-// cycles for (2 to 4 per cent of the time).  2,048 tokens behind 14,336 (32 heads on 8): 442 to 458 us, 1,125 to 1,166 TFLOP/s where an 8192^3
+// cycles for (2 to 4 per cent of the time).  2,048 tokens behind 14,336 (32 heads on 8): 442 to 467 us, 1,104 to 1,166 TFLOP/s where an 8192^3
 // bf16 product reaches 1,212; 16-bit pages 535.  Keys read by every wave from memory, without LDS, took 1,561.  A ring of four rounds in LDS was
 // 3 to 20 per cent slower (room for fewer workgroups), a round's weighted values under the next round's softmax 15 (spills), widening between
 // the weighted values' products and wave priorities no different.
@@ -1397,7 +1403,8 @@ extern "C" int as_qk_norm_rope_store8(const void* qkv, const void* qw, const voi
   if (R == 0) cs = nullptr;
   // Tokens whose runs a wave takes: 16 is a block, so that a prompt's waves have one run each, but single tokens, four at a time, are a chain of up to four
   // turns then.  us with 4 / 8 / 16, 32 heads of 128 on 8: single tokens of 64 requests 4.0 / 4.9 / 6.8, of 256 4.8 / 5.7 / 7.4, of 512 6.7 / 6.5 / 8.1; prompts
-  // of 512 5.4 / 5.0 / 4.9, of 2,048 17.5 / 14.0 / 11.8, of 480 beside 32 single tokens 5.5 / 5.2 / 7.0.
+  // of 512 5.4 / 5.0 / 4.9, of 2,048 17.5 / 14.0 / 11.8, of 480 beside 32 single tokens 5.5 / 5.2 / 7.0.  Other widths and
+  // numbers of kv heads go by the same number of (token, kv head) pairs and were not swept.
   const long long pairs = (long long)num_tokens * KV;
   const int chunk = pairs <= 2048 ? 4 : pairs <= 6144 ? 8 : 16;
   const long long kv_blocks = store ? (((long long)num_tokens + chunk - 1) / chunk * 2 * KV + 3) / 4 : 0;

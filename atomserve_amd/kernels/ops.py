@@ -787,7 +787,8 @@ def attn_mixed(q, k_pages, v_pages, items, tiles, positions, tok_row, block_tabl
 #
 # Keys and values as e4m3 numbers in blocks of 16 tokens; for every block and kv head one scale for the keys and one for the values: the power of
 # two 2^e with the smallest e in -100 .. 119 for which the block's largest magnitude is at most 448 * 2^e.  Half of a bfloat16 cache's bytes: twice
-# the tokens in the same memory, and half of what the attention of single queries waits for.  A number is off by at most 2^-4 of itself.
+# the tokens in the same memory, and half of what the attention of single queries waits for.  A number is off by at most 2^-4 of itself; under
+# 2^-6 of its block's scale (2^-14 of the block's largest) by up to 2^-9 of the scale, since it is rounded again whenever the scale grows.
 #
 #   k_pages  [num_pages, KV, block_size, D]             float8_e4m3fn
 #   v_pages  [num_pages, KV, block_size / 16, D, 16]    float8_e4m3fn (a block's values are transposed)
