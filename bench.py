@@ -96,7 +96,10 @@ def parse_args():
                    help="also split the host's time of a decode step into schedule / pack / launch / sample / wait / "
                         "update (steps run one at a time meanwhile, none sent ahead), as the reference's "
                         "bench/engine.py --profile does")  # fmt: skip
-    return p.parse_args()
+    args = p.parse_args()
+    if args.cache_bits == 8 and (args.design != "qwen3" or args.dtype != "bf16" or args.block_size % 16):
+        p.error("--cache-bits 8 is for the Qwen3 layers in bf16, with pages of a multiple of 16 tokens")
+    return args
 
 
 def prompt(b: int, n: int, vocab: int) -> list:

@@ -28,3 +28,19 @@ def test_results_that_are_no_tensor_are_refused(call, out):
 def test_single_queries_without_heads_are_refused():
     with pytest.raises(ops.KernelError, match="heads 0/2"):
         single(H=0)
+
+
+@pytest.mark.parametrize("wrong", [["--design", "dozusun"], ["--design", "tokuvik"], ["--dtype", "fp32"], ["--block-size", "8"]])
+def test_a_benchmark_that_would_not_hold_its_cache_in_8_bits_is_refused(monkeypatch, capsys, wrong):
+    import sys
+
+    import bench
+
+    monkeypatch.setattr(sys, "argv", ["bench.py", "--cache-bits", "8"])
+    assert bench.parse_args().cache_bits == 8
+    monkeypatch.setattr(sys, "argv", ["bench.py", *wrong])
+    assert bench.parse_args().cache_bits == 0
+    monkeypatch.setattr(sys, "argv", ["bench.py", "--cache-bits", "8", *wrong])
+    with pytest.raises(SystemExit):
+        bench.parse_args()
+    assert "--cache-bits 8" in capsys.readouterr().err
