@@ -414,7 +414,7 @@ template <int D, typename W> __global__ __launch_bounds__(256) void append8_kern
 //                                split in two e4m3 parts, the number rounded and what is left of it: 4 + 4 bits hold a bf16 number's eight
 //                                exactly, down to 2^-9.8 of the query's largest coordinate, and what is smaller is off by 2^-17.8 of it at most
 //                                (half a smallest step, 2^-10, where the largest is 224 or more).
-//   softmax                      fp32, base 2, maxima and sums kept per column
+//   softmax                      fp32, base 2, what weights are relative to and their sums kept per column
 //   O^T[d][column] += V^T P^T    values as bf16 (exact, the scale included), weights rounded to bf16: the matrix cores' operands, a part of 2^-8 at most
 //
 // The denominator is the 32-bit sum of the weights: as they are for single queries, rounded for portions, where the matrix cores add them up.  Either way a
@@ -427,9 +427,15 @@ constexpr int STEP = 64;
 template <int D> struct Query {
   u32x4_t high[D / 64], low[D / 64];  // coordinates 64 c + 16 grp .. + 15 of this lane's column
   float scale;
+  float sum;  // what the sum of its weights begins with
+  // No e4m3 numbers stand for a query that is not finite.  Its scores count as 0, so that they move no maximum, and its sum is NaN: its result
+  // is, and none of its neighbours'.
+  __device__ __forceinline__ void finite_or_not(float amax) {
+    const bool finite = amax < __builtin_inff();
+    scale = finite ? scale : 0.f;
+    sum = finite ? 0.f : __builtin_nanf("");
+  }
 };
-
-constexpr unsigned FOUR_NANS = 0x7f7f7f7fu;  // what a query that is not finite is made of: its scores become NaN, and none of its neighbours'
 
 // Four numbers of a query, scaled, as their two parts.
 __device__ __forceinline__ void split4(const float* x, float inv, unsigned& high, unsigned& low) {
@@ -455,16 +461,16 @@ template <int D> __device__ __forceinline__ void load_query(Query<D>& q, const b
   const float amax = quad_rows_max(__uint_as_float(min(most, 0x7f800000u)));
   q.scale = block_scale(amax);
   const float inv = inverse_of(q.scale);
-  const bool finite = amax < __builtin_inff();
 #pragma unroll
   for (int c = 0; c < D / 64; ++c)
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       unsigned high, low;
       split4(x[c] + 4 * w, inv, high, low);
-      q.high[c][w] = finite ? high : FOUR_NANS;
+      q.high[c][w] = high;
       q.low[c][w] = low;
     }
+  q.finite_or_not(amax);
 }
 
 __device__ __forceinline__ i32x8_t both(u32x4_t a, u32x4_t b) {
@@ -487,20 +493,28 @@ template <int D> __device__ __forceinline__ f32x4_t score_tile(const u32x4_t (&k
   return s;
 }
 
-// What scores are taken relative to need not be their maximum: weights of up to 2 are as good as those of up to 1.  So a maximum that has grown by no more than a
-// factor of 2 moves nothing, and whether one has grown by more is all that a step asks; lanes agree on a new one, and sums are rescaled, only then.  2,048
+// What scores are taken relative to need not be their maximum: half of it is as good.  So the reference is SLACK (a factor of 2) above the maximum that moved it
+// last, a maximum up to there moves nothing, and whether one is beyond is all that a step asks; lanes agree on a new one, and sums are rescaled, only then.  2,048
 // tokens behind 14,336 take 458 us, 485 where every step does all of it, 472 where it does so for any growth and 445 where it does so for a growth beyond 2^8;
-// but a largest weight that is not 1 is rounded to bfloat16 itself: errors against 64 bits are 1.93e-3, 1.88e-3, 1.88e-3 and 2.12e-3.
+// but a largest weight that is no power of two is rounded to bfloat16 itself: errors against 64 bits are 1.93e-3, 1.88e-3, 1.88e-3 and 2.12e-3.
+//
+// A weight is 2^(score x factor - reference) by one fused operation, whose product is not rounded, while a maximum is a rounded product: from 2^22 on the two are
+// up to a quarter apart and more, from 2^31 on a weight would be infinite, or all of them 0.  There the reference is 2 to 4 steps below the maximum instead, and weights,
+// which are 1 at most anyway, are cut at 1 by the exponential's own clamp, which is free: what 32 bits hardly tell from the maximum weighs as much.
 constexpr float SLACK = 1.f;  // in base 2
+__device__ __forceinline__ float reference_of(float top) { return fabsf(top) < 0x1p22f ? top + SLACK : top - fabsf(top) * 0x1p-22f; }
+__device__ __forceinline__ float weight_of(float score, float by, float base) {
+  return __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(fmaf(score, by, -base)), 0.f, 1.f);
+}
 
 template <int D> struct Running {
   f32x4_t o[D / 16];
-  float m, l;  // the column's maximum (base 2) or up to SLACK less, and the sum of this lane's weights
-  __device__ __forceinline__ void clear() {
+  float m, l;  // the column's reference (base 2; -inf: nothing seen), and the sum of this lane's weights
+  __device__ __forceinline__ void clear(const Query<D>& q) {
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) o[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     m = NEG_INF;
-    l = 0.f;
+    l = q.sum;
   }
 };
 
@@ -604,8 +618,8 @@ __device__ __forceinline__ void take_step(const Held<D>& held, int kb, const Que
       }
   }
   const float top = max_of_16(s) * by;
-  if (__any(top > run.m + SLACK)) {  // uniform; rare once the first keys have been seen
-    const float mn = fmaxf(run.m, quad_rows_max(top));
+  if (__any(top > run.m)) {  // uniform; rare once the first keys have been seen
+    const float mn = fmaxf(run.m, reference_of(quad_rows_max(top)));
     const float alpha = __builtin_amdgcn_exp2f(run.m - (mn == NEG_INF ? 0.f : mn));
     run.m = mn;
     run.l *= alpha;
@@ -619,7 +633,7 @@ __device__ __forceinline__ void take_step(const Held<D>& held, int kb, const Que
   for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const float w = __builtin_amdgcn_exp2f(fmaf(s[tt][r], by, -base));
+      const float w = weight_of(s[tt][r], by, base);
       sum[r] += w;
       p[tt >> 1][(tt & 1) * 4 + r] = (bf16)w;
     }
@@ -688,7 +702,7 @@ __device__ __forceinline__ float share_of(const Sight& sight, int head, float m,
     if (top == NEG_INF) return 0.f;  // a sink of no weight, beside nothing
     return e / (l * e + __builtin_amdgcn_exp2f(sk - top));
   }
-  return l > 0.f ? 1.0f / l : 0.f;
+  return l == 0.f ? 0.f : 1.0f / l;
 }
 
 // FRESH: the kernel takes the projection's output instead of finished queries and does what `append8_kernel` does before a decode step whose tokens are
@@ -703,8 +717,8 @@ struct Fresh {
 // A query as the lanes that normed it leave it in LDS: the parts that `load_query` makes.
 template <int D> struct Split {
   unsigned high[D / 4], low[D / 4];
-  float scale;
-  unsigned apart[3];
+  float scale, amax;
+  unsigned apart[2];
 };
 
 // The token's key and value as its block holds them, in LDS.
@@ -843,8 +857,6 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a
     load_step<D>(even, a.pages, blocks, page_head);
     if (at + 4 < to) blocks.ask(a.pages, pieces, steps.first_key(at + 4));
   }
-  Running<D> run;
-  run.clear();
   Query<D> q;
   [[maybe_unused]] News<D>* const news = reinterpret_cast<News<D>*>(smem + 128 + 4 * LD * G);
   if constexpr (FRESH) {
@@ -877,15 +889,12 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a
         const float amax = lanes_max<LPT>(busy ? __uint_as_float(min(most, 0x7f800000u)) : 0.f), scale = block_scale(amax), inv = inverse_of(scale);
         if (!busy) continue;
         Split<D>& to8 = queries[job];
-        unsigned high[2], low[2];
-        split4(x, inv, high[0], low[0]);
-        split4(x + 4, inv, high[1], low[1]);
-        const bool finite = amax < __builtin_inff();
-        to8.high[at8.a / 4] = finite ? high[0] : FOUR_NANS;
-        to8.high[at8.b / 4] = finite ? high[1] : FOUR_NANS;
-        to8.low[at8.a / 4] = low[0];
-        to8.low[at8.b / 4] = low[1];
-        if (j == 0) to8.scale = scale;
+        split4(x, inv, to8.high[at8.a / 4], to8.low[at8.a / 4]);
+        split4(x + 4, inv, to8.high[at8.b / 4], to8.low[at8.b / 4]);
+        if (j == 0) {
+          to8.scale = scale;
+          to8.amax = amax;
+        }
       } else {
         float amax = 0.f;
 #pragma unroll
@@ -913,10 +922,13 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a
       q.low[c] = *reinterpret_cast<const u32x4_t*>(&from8.low[16 * c + 4 * grp]);
     }
     q.scale = from8.scale;
+    q.finite_or_not(from8.amax);
   } else {
     load_query<D>(q, a.q + ((size_t)t * a.H + h0 + min(col, G - 1)) * D, grp);
   }
   const float factor = score_factor(a) * q.scale;
+  Running<D> run;
+  run.clear(q);
   auto turn = [&](Held<D>& now, Held<D>& next) {
     if constexpr (FRESH) {
       if (here && at == last) {  // uniform: this wave's step holds the token itself
@@ -936,7 +948,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void single8_kernel(Attend a
   }
   run.l = quad_rows_sum(run.l);
   float *sm = smem, *sl = smem + 64, *so = smem + 128;
-  if (grp == 0 && col < G) { sm[wave * 16 + col] = run.m; sl[wave * 16 + col] = run.l; }
+  if (grp == 0 && col < G) { sm[wave * 16 + col] = run.m; sl[wave * 16 + col] = run.m == NEG_INF ? 0.f : run.l; }
   if (col < G)
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f32x4_t*>(so + (wave * G + col) * LD + d * 16 + 4 * grp) = run.o[d];
@@ -1028,7 +1040,7 @@ __global__ __launch_bounds__(256) void single8_merge_kernel(Attend a, int D) {
 struct Cut {
   int pieces, piece_rounds;
   int* cut;    // [items]: the pieces of each (1: not cut)
-  float* ml;   // [T, H, pieces, 2] maximum (base 2), sum
+  float* ml;   // [T, H, pieces, 2] what weights are relative to (base 2), sum
   float* acc;  // [T, H, pieces, D]
 };
 
@@ -1109,21 +1121,21 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt8_kernel(Attend a
   Running<D> run[QT];
   int qpos[QT], qlo[QT];
   float factor[QT];
-  float base[QT];  // the columns' maxima; 0 while there is none
+  float base[QT];  // the columns' references; 0 while there is none
   f32x4_t l[QT];  // sums of weights, the same in every row: the weights' product with ones
   bf16x8_t ones;
 #pragma unroll
   for (int i = 0; i < 8; ++i) ones[i] = (bf16)1.f;
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
-    l[qt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     base[qt] = 0.f;
     const int qc = min(qt * 16 + col, nq - 1);  // columns past the end repeat the last query and are not stored
     qpos[qt] = min(pos0 + q0 + qc, end);
     qlo[qt] = first_seen(qpos[qt]);
     load_query<D>(q[qt], a.q + ((size_t)(tok0 + (working ? q0 + qc : 0)) * a.H + head) * D, grp);
     factor[qt] = score_factor(a) * q[qt].scale;
-    run[qt].clear();
+    run[qt].clear(q[qt]);
+    l[qt] = f32x4_t{run[qt].l, run[qt].l, run[qt].l, run[qt].l};
   }
 
   // where blocks lie: lane l has block l % 4 of round 16 batch + l / 4
@@ -1247,12 +1259,12 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt8_kernel(Attend a
             }
         }
         top[qt] = max_of_16(s[qt]) * by[qt];
-        grows = grows || top[qt] > run[qt].m + SLACK;
+        grows = grows || top[qt] > run[qt].m;
       }
       if (__any(grows)) {  // uniform; rare once the first keys have been seen
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
-          const float mn = fmaxf(run[qt].m, quad_rows_max(top[qt]));
+          const float mn = fmaxf(run[qt].m, reference_of(quad_rows_max(top[qt])));
           base[qt] = mn == NEG_INF ? 0.f : mn;
           const float alpha = __builtin_amdgcn_exp2f(run[qt].m - base[qt]);
           run[qt].m = mn;
@@ -1266,7 +1278,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt8_kernel(Attend a
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) p[qt][tt >> 1][(tt & 1) * 4 + r] = (bf16)__builtin_amdgcn_exp2f(fmaf(s[qt][tt][r], by[qt], -base[qt]));
+          for (int r = 0; r < 4; ++r) p[qt][tt >> 1][(tt & 1) * 4 + r] = (bf16)weight_of(s[qt][tt][r], by[qt], base[qt]);
       if constexpr (!EARLY) read_values(0);
       read_values(1);
       __builtin_amdgcn_sched_barrier(0);

@@ -98,6 +98,37 @@ def test_a_key_that_is_not_seen_yet_is_far_larger_than_all_that_is(ops, monkeypa
     check_all(ops, monkeypatch, torch.full((L, H, D), 2.0**40, device=DEV).to(BF16), cache, table, visible=8, **kw)
 
 
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("D", [64, 128, 192, 256])
+@pytest.mark.parametrize("exponent", [8, 14, 18, 30, 50])
+def test_scores_of_any_size_that_32_bits_hold(ops, monkeypatch, D, exponent, sign):
+    """Scores of up to 2^100, all of them above or all below zero, far enough apart that the largest weighs 1 and the others nothing: the value of that key."""
+    L, H, KV = 100, 4, 2
+    g = torch.Generator(device=DEV).manual_seed(exponent)
+    keys = (1 + torch.randperm(L, generator=g, device=DEV)[:, None, None] / 8.0).expand(L, KV, D) * 2.0**exponent
+    cache, table = one_request(L, H, KV, D, 16, keys)
+    k, v = plain.gathered(cache, table, L)  # as 8-bit numbers a sixteenth of themselves apart, or the same
+    q = torch.full((L, H, D), sign * 1.3 * 2.0**exponent, device=DEV).to(BF16)
+    scores = (k.sum(-1) * float(q[0, 0, 0]))[0]
+    want = torch.stack([v[:, : p + 1][:, scores[: p + 1] == scores[: p + 1].max()].mean(1) for p in range(L)])  # [L, KV, D]
+    want = want.repeat_interleave(H // KV, 1)
+
+    def check(out, name):  # equal keys weigh the same: their mean, by a weight rounded to bfloat16 over one that is not, and rounded itself
+        assert bool(out.isfinite().all()), name
+        assert bool(((out.double() - want).abs() <= 2.0**-7 * (1 + 2.0**-7) * want.abs() + 2.0**-20).all()), name
+
+    scale, tables = plain.default_scale(D), i32([table])
+    for part in (64, 4096):
+        out = torch.full_like(q, 7.0)
+        ops.attn_single_query8(q, *cache, None, i32(range(L)), torch.zeros(L, dtype=I32, device=DEV), tables, out, scale, 0, L, part_size=part)
+        check(out, f"partitions of {part}")
+    for query_tiles, pieces in ((1, 1), (2, 2)):
+        monkeypatch.setattr(ops, "PREFILL_PIECES", pieces)
+        out = torch.full_like(q, 7.0)
+        ops.attn_prefill8(q, *cache, i32([(0, 64, 0, 0), (64, 36, 0, 64)]), tables, out, scale, 0, L, query_tiles=query_tiles)
+        check(out, f"{query_tiles} tiles a wave, {pieces} pieces")
+
+
 @pytest.mark.parametrize("D", [64, 128, 192])
 @pytest.mark.parametrize("context", [1, 2, 16, 17, 64, 70])
 def test_a_decode_step_of_zeros(ops, D, context):
