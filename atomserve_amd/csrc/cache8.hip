@@ -498,11 +498,11 @@ template <int D> __device__ __forceinline__ f32x4_t score_tile(const u32x4_t (&k
 // tokens behind 14,336 take 458 us, 485 where every step does all of it, 472 where it does so for any growth and 445 where it does so for a growth beyond 2^8;
 // but a largest weight that is no power of two is rounded to bfloat16 itself: errors against 64 bits are 1.93e-3, 1.88e-3, 1.88e-3 and 2.12e-3.
 //
-// A weight is 2^(score x factor - reference) by one fused operation, whose product is not rounded, while a maximum is a rounded product: from 2^22 on the two are
-// up to a quarter apart and more, from 2^31 on a weight would be infinite, or all of them 0.  There the reference is 2 to 4 steps below the maximum instead, and weights,
+// A weight is 2^(score x factor - reference) by one fused operation, whose product is not rounded, while a maximum is a rounded product: from 2^24 on the two are
+// up to SLACK apart and more, from 2^31 on a weight would be infinite, or all of them 0.  There the reference is 2 to 4 steps below the maximum instead, and weights,
 // which are 1 at most anyway, are cut at 1 by the exponential's own clamp, which is free: what 32 bits hardly tell from the maximum weighs as much.
 constexpr float SLACK = 1.f;  // in base 2
-__device__ __forceinline__ float reference_of(float top) { return fabsf(top) < 0x1p22f ? top + SLACK : top - fabsf(top) * 0x1p-22f; }
+__device__ __forceinline__ float reference_of(float top) { return fabsf(top) < 0x1p24f ? top + SLACK : top - fabsf(top) * 0x1p-22f; }
 __device__ __forceinline__ float weight_of(float score, float by, float base) {
   return __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(fmaf(score, by, -base)), 0.f, 1.f);
 }

@@ -129,6 +129,31 @@ def test_scores_of_any_size_that_32_bits_hold(ops, monkeypatch, D, exponent, sig
         check(out, f"{query_tiles} tiles a wave, {pieces} pieces")
 
 
+@pytest.mark.parametrize("common", [0, 2**10, 2**20, 2**23, 2**25])
+def test_two_large_scores_that_are_a_little_apart(ops, common):
+    """Scores of `common` and 4 more: the factor is the same for both, and a fused product minus a maximum keeps their distance, up to 2^24 in base 2; beyond, what
+    comes out lies between the two values."""
+    H, KV, D, L = 2, 1, 64, 2
+    keys = torch.zeros(L, KV, D, device=DEV)
+    keys[:, 0, 0], keys[1, 0, 8] = 256.0, 1.0  # not among the same eight coordinates, whose products are aligned to the largest
+    cache, table = one_request(L, H, KV, D, 16, keys)
+    q = torch.zeros(L, H, D, device=DEV)
+    q[:, :, 0], q[:, :, 8] = common / 32, 32.0  # all powers of two: exact in 8 bits, also beside one another
+    q = q.to(BF16)
+    k, v = plain.gathered(cache, table, L)
+    assert torch.equal(k[0], keys[:, 0].double())
+    want = (torch.softmax(torch.tensor([0.0, 4.0], dtype=F64), 0).to(DEV)[:, None] * v[0]).sum(0)
+    outs = [torch.full((L, H, D), 7.0, dtype=BF16, device=DEV) for _ in range(3)]
+    for part, out in zip((64, 4096), outs):
+        ops.attn_single_query8(q, *cache, None, i32(range(L)), i32([0] * L), i32([table]), out, 0.125, 0, L, part_size=part)
+    ops.attn_prefill8(q, *cache, i32([(0, 2, 0, 0)]), i32([table]), outs[2], 0.125, 0, L)
+    for out in outs:
+        got = out[1].double()
+        if common <= 2**23:  # weights and the result are rounded to bfloat16
+            assert bool(((got - want).abs() <= 2.0**-7 * v[0].abs().sum(0)).all())
+        assert bool(((got >= v[0].amin(0) - 2.0**-7 * v[0].abs().sum(0)) & (got <= v[0].amax(0) + 2.0**-7 * v[0].abs().sum(0))).all())
+
+
 @pytest.mark.parametrize("D", [64, 128, 192])
 @pytest.mark.parametrize("context", [1, 2, 16, 17, 64, 70])
 def test_a_decode_step_of_zeros(ops, D, context):
