@@ -797,6 +797,7 @@ def attn_mixed(q, k_pages, v_pages, items, tiles, positions, tok_row, block_tabl
 # Slots and block tables are those of a 16-bit cache.  Blocks start on 16 bytes, as do the other tensors of these calls.  What a block holds is known once its first place is written: a call that writes the first place
 # makes the block new and forgets what it held, and a call that goes on in a block lets its scale grow and rewrites it.  Pools start zeroed
 # (what a mask hides is multiplied by zero, so it has to be a number): what is not finite is never stored.  A query that is not finite gives NaN.
+# Scores are products of the 8-bit numbers as they are; of every eight neighbouring coordinates those far below the largest lose bits: up to 2^-10 of it in all.
 
 E4M3 = torch.float8_e4m3fn
 BLOCK8 = 16  # tokens that share a scale

@@ -208,6 +208,71 @@ def test_queries_that_are_not_finite_are_nan_and_their_neighbours_are_not(ops, m
                                                         out, H, scale, 0, L, part_size=part), q, bad, hit)  # fmt: skip
 
 
+# ---- products beside far larger ones --------------------------------------------------------------------
+
+
+def exponents(x):
+    """The exponents of numbers as e4m3 numbers have them (-6 under the smallest normal one); of zeros, one that nothing is aligned to."""
+    return torch.where(x == 0, -1000, torch.floor(torch.log2(x.abs().clamp(min=2.0**-6))))
+
+
+def scores_as_cut(q, k8):
+    """q [H, D] (bfloat16 numbers) and k8 [L, D] (e4m3 numbers): the products' sums as the matrix cores take them, [H, L].  A query, scaled by a power of two,
+    is two e4m3 parts; of either part's products, those of eight neighbouring coordinates are cut, towards zero, to multiples of 2^-13 of the
+    largest exponent's power of two among them."""
+    amax = q.abs().amax(-1)
+    scale = torch.tensor([plain.scale_of(float(x)) for x in amax], dtype=F64, device=q.device)[:, None]
+    y = q / scale
+    high = y.float().to(torch.float8_e4m3fn).double()
+    low = (y - high).float().to(torch.float8_e4m3fn).double()
+    total = 0
+    for part in (high, low):
+        products = (part[:, None] * k8[None]).unflatten(-1, (-1, 8))
+        e = (exponents(part)[:, None] + exponents(k8)[None]).unflatten(-1, (-1, 8))
+        step = 2.0 ** (e.amax(-1, keepdim=True).clamp(min=-200) - 13)
+        total = total + (torch.trunc(products / step) * step).sum((-1, -2))
+    return total * scale
+
+
+@pytest.mark.parametrize("D", [64, 128, 192, 256])
+@pytest.mark.parametrize("offset,places", [(0, 1), (30, 1), (30, 4), (100, 1), (100, 4), (300, 1), (1000, 4)])
+def test_scores_beside_a_coordinate_that_is_far_larger_than_the_others(ops, D, offset, places):
+    """Heads with a coordinate that adds much to every score: attention with the scores that the matrix cores make of such products, to the roundings that there are
+    everywhere else; and those scores within 2^-10 of the largest product of every eight of the definition's."""
+    L, H, KV, bs = 150, 2, 1, 16
+    g = torch.Generator(device=DEV).manual_seed(D + offset)
+    keys, q = torch.randn(L, KV, D, generator=g, device=DEV), torch.randn(L, H, D, generator=g, device=DEV)
+    large = (offset * D**0.5 / places) ** 0.5
+    for i in range(places):
+        if offset:
+            keys[..., 5 + 12 * i] = large * (1 + 0.01 * torch.randn(L, KV, generator=g, device=DEV))
+            q[..., 5 + 12 * i] = large
+    cache, table = one_request(L, H, KV, D, bs, keys)
+    q, scale, tables = q.to(BF16), plain.default_scale(D), i32([table])
+    single, portion = torch.full_like(q, 7.0), torch.full_like(q, 7.0)
+    ops.attn_single_query8(q, *cache, None, i32(range(L)), torch.zeros(L, dtype=I32, device=DEV), tables, single, scale, 0, L)
+    ops.attn_prefill8(q, *cache, i32([(at, min(64, L - at), 0, at) for at in range(0, L, 64)]), tables, portion, scale, 0, L)
+    k, v = plain.gathered(cache, table, L)
+    k_scales = cache[2][: -(-L // bs), 0].double().flatten().repeat_interleave(16)[:L]
+    k8 = k[0] / k_scales[:, None]
+    for p in (*range(0, L, 7), L - 1):
+        seen, x = slice(0, p + 1), q[p].double()
+        cut = scores_as_cut(x, k8[seen]) * k_scales[None, seen]
+        exact = x @ k[0, seen].T
+        most = (x.abs()[:, None] * k[:, seen].abs()).unflatten(-1, (-1, 8)).amax(-1)
+        small = x.abs().amax(-1, keepdim=True) * 2.0**-10 / 224 * k[0, seen].abs().sum(-1)  # the query's second part
+        assert bool(((cut - exact).abs() <= 2.0**-10 * most.sum(-1) + small).all())
+        s = cut * scale
+        w = torch.softmax(s, -1)
+        want, size = w @ v[0, seen], w @ v[0, seen].abs()
+        # weights and the result rounded to bfloat16, the portions' denominator of rounded weights; sums across groups of eight, the factor and the
+        # exponent in 32 bits: 2^-20 of the products' magnitudes, twice
+        off = 2.0**-20 * scale * (x.abs() @ k[0, seen].abs().T).amax(-1, keepdim=True) + 2.0**-20 * s.abs().amax(-1, keepdim=True)
+        bound = 2.0**-8 * (1 + 2.0**-7) * (size + 2 * want.abs()) + (2 * off + 2.0**-16) * size + 1e-30
+        for out, name in ((single, "single"), (portion, "portion")):
+            assert bool(((out[p].double() - want).abs() <= bound).all()), (name, p, float(((out[p].double() - want).abs() / bound).max()))
+
+
 # ---- heads whose lanes are not all at work --------------------------------------------------------------
 
 
